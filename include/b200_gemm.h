@@ -255,6 +255,90 @@ int b200_gemm_slab_gather(int types, void* const* C_full, const void* A, const v
 int b200_gemm_slab_host(b200_gemm_comm* comm, int types, void* C_slab, const void* A, const void* B_slab, size_t M,
                         size_t N, size_t K, int layout_c, int layout_a, int layout_b, size_t align);
 
+/* ---- products with epilogues, grouped products, and their gradients -------------------------
+ * What a layer does around its product, in the product's own kernel.  No counterpart in the
+ * reference, which computes C = A * B alone.
+ *
+ *   forward    Z = A*B + bias        C = act(Z) + residual
+ *   gradient   C = (A*B) .* act'(Z)  bias_grad = column sums of C (before C is rounded)
+ *
+ * Everything after the product is computed in f32 from the f32 accumulators and rounded once,
+ * when C and Z are stored: C is rounded from act of the unrounded Z, the gradient takes the
+ * stored (rounded) Z.  The bias gradient is always f32, summed in a fixed order (equal inputs give
+ * equal bits).  bias, residual, preact and C share C's element type; residual and preact are
+ * matrices of C's shape, layout and batch stride.
+ *
+ * The calls are asynchronous on `*stream`, on the current device, and may be captured into a
+ * graph after the first call on the device.  A call that needs scratch memory (bias gradients, K
+ * partitions, operands that have to be padded) keeps it per stream and lets it grow on demand; a
+ * captured call's scratch belongs to the graph.  Calls that overlap on the GPU must not share
+ * outputs; host threads must not issue calls on one stream at the same time.
+ *
+ * Refused before anything runs: bad layouts, sizes, activations (BAD_LAYOUT, BAD_SIZE, BAD_CONFIG),
+ * missing pointers (NULL_POINTER), pointers not aligned to their element (MISALIGNED), a bias,
+ * residual or bias_grad in the mode that does not take it, and outputs that overlap other
+ * arguments (BAD_CONFIG) - except C with residual, and C with preact in gradient mode, which
+ * may be the same buffer (in place). */
+enum b200_gemm_activation {
+    B200_GEMM_ACT_NONE      = 0,
+    B200_GEMM_ACT_RELU      = 1,
+    B200_GEMM_ACT_SILU      = 2, /* x sigmoid(x) */
+    B200_GEMM_ACT_GELU_TANH = 3, /* x/2 (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
+    B200_GEMM_ACT_GELU      = 4  /* x/2 (1 + erf(x / sqrt 2)) */
+};
+
+typedef struct b200_gemm_epilogue {
+    int         activation;  /* b200_gemm_activation */
+    int         gradient;    /* 0: forward, 1: gradient */
+    const void* bias;        /* forward: NULL, or N values (one per column of C) */
+    const void* residual;    /* forward: NULL, or a matrix like C; may be C itself */
+    void*       preact;      /* forward: NULL, or where Z is stored; gradient: Z (NULL only with
+                                B200_GEMM_ACT_NONE); may be C itself in gradient mode */
+    float*      bias_grad;   /* gradient: NULL, or N sums over the rows of C */
+    size_t      bias_stride; /* batched calls: elements between the biases (and bias gradients) of
+                                consecutive items; 0 = one bias for all items, whose gradient is the
+                                sum over all items.  Otherwise at least N.  Grouped calls: ignored,
+                                bias and bias_grad are groups x N. */
+} b200_gemm_epilogue;
+
+/* C = A*B with an epilogue (epi NULL: none).  Arguments as in b200_gemm_ex.  M, N, K, batch of 0:
+ * empty C is left alone, a bias gradient over no rows is zero, K == 0 is a product of zeros
+ * (the epilogue still applies).  The plan is that of b200_gemm_ex for the same problem. */
+int b200_gemm_fused(int types, void* C, const void* A, const void* B, size_t M, size_t N, size_t K,
+                    size_t batch_count, int layout_c, int layout_a, int layout_b, void* stream,
+                    const b200_gemm_epilogue* epi);
+
+/* Grouped product (experts): A (rows x K) and C (rows x N) are row-major, group e owns the rows
+ * [offsets[e], offsets[e+1]) and has its own K x N matrix B + e*K*N in layout_b:
+ *   C[rows of e] = epilogue(A[rows of e] * B_e)
+ * `offsets` is an array of groups + 1 ints ON THE DEVICE, read by the kernel: non-decreasing, within
+ * [0, rows].  Groups may be empty.  Rows before offsets[0] and from offsets[groups] on belong to no
+ * group: they are neither read into any result nor written (C, preact).  bias and bias_grad are
+ * groups x N; an empty group's bias gradient is zero.  Offsets outside the rule are taken as their
+ * running maximum clamped to [0, rows]: no access leaves the matrices.  1 <= groups <= 1024.
+ * The input gradient of the product is this call on dC with layout_b flipped (B_e^T is the N x K
+ * matrix of the other layout) and N and K exchanged. */
+#define B200_GEMM_MAX_GROUPS 1024
+int b200_gemm_grouped(int types, void* C, const void* A, const void* B, const int* offsets, size_t rows,
+                      size_t N, size_t K, size_t groups, int layout_b, void* stream,
+                      const b200_gemm_epilogue* epi);
+
+/* Weight gradient of a grouped product: A (rows x M) and B (rows x N) row-major,
+ *   C_e (M x N, layout_c, at C + e*M*N) = A[rows of e]^T * B[rows of e]   (+ C_e with accumulate != 0)
+ * An empty group's C_e is zero (or left as it is with accumulate).  offsets and groups as above. */
+int b200_gemm_grouped_wgrad(int types, void* C, const void* A, const void* B, const int* offsets, size_t rows,
+                            size_t M, size_t N, size_t groups, int layout_c, int accumulate, void* stream);
+
+/* Backward through an activation where no product precedes it:
+ *   dZ = dY .* act'(Z)      bias_grad = column sums of dZ (before dZ is rounded)
+ * for M x N matrices of one element type, that of the C of `types`, all in `layout`.  dZ may be
+ * NULL (only the sums), dY or Z itself; preact may be NULL with B200_GEMM_ACT_NONE.  With offsets
+ * (groups > 0, layout 0, batch_count 1) the rows are ragged as above: bias_grad is groups x N,
+ * and rows that belong to no group are left as they are.  bias_stride as in b200_gemm_epilogue. */
+int b200_gemm_activation_backward(int types, void* dZ, const void* dY, const void* preact, size_t M, size_t N,
+                                  size_t batch_count, int layout, int activation, float* bias_grad,
+                                  size_t bias_stride, const int* offsets, size_t groups, void* stream);
+
 /* Bytes of f32 split-K workspace a call would use (0 when the chosen config has split_k 1). */
 size_t b200_gemm_workspace_bytes(int types, size_t M, size_t N, size_t K, size_t batch_count,
                                  int layout_c, int layout_a, int layout_b,

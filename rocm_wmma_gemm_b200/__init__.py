@@ -21,7 +21,7 @@ from . import build as _build
 
 __all__ = [
     "m_layout", "loader", "GemmConfig", "GemmError", "lib", "get_gemm_params", "slab",
-    "TYPE_PAIRS", "ABI_SYMBOLS", "device_status", "static_status", "launch_count", "plan", "PlanInfo", "RASTER_SNAKE",
+    "Epilogue", "ACTIVATIONS", "MAX_GROUPS", "TYPE_PAIRS", "ABI_SYMBOLS", "device_status", "static_status", "launch_count", "plan", "PlanInfo", "RASTER_SNAKE",
 ]
 
 
@@ -47,6 +47,18 @@ class GemmConfig(ctypes.Structure):
 
     def __repr__(self) -> str:
         return "GemmConfig(" + ", ".join(f"{k}={v}" for k, v in self.as_dict().items()) + ")"
+
+
+class Epilogue(ctypes.Structure):
+    """Mirror of `b200_gemm_epilogue` (include/b200_gemm.h)."""
+    _fields_ = [("activation", ctypes.c_int), ("gradient", ctypes.c_int), ("bias", ctypes.c_void_p),
+                ("residual", ctypes.c_void_p), ("preact", ctypes.c_void_p), ("bias_grad", ctypes.c_void_p),
+                ("bias_stride", ctypes.c_size_t)]
+
+
+# Activation names -> b200_gemm_activation
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "gelu": 4}
+MAX_GROUPS = 1024  # B200_GEMM_MAX_GROUPS
 
 
 class PlanInfo(ctypes.Structure):
@@ -118,6 +130,15 @@ ABI_SYMBOLS = {
                                              ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_int, ctypes.c_int,
                                              ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p,
                                              ctypes.POINTER(GemmConfig)]),
+    # products with epilogues, grouped products, gradients
+    "b200_gemm_fused": (ctypes.c_int, [ctypes.c_int] + _GEMM_ARGS + [ctypes.POINTER(Epilogue)]),
+    "b200_gemm_grouped": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_void_p] * 4 + [ctypes.c_size_t] * 4
+                          + [ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(Epilogue)]),
+    "b200_gemm_grouped_wgrad": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_void_p] * 4 + [ctypes.c_size_t] * 4
+                                + [ctypes.c_int, ctypes.c_int, ctypes.c_void_p]),
+    "b200_gemm_activation_backward": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_void_p] * 3 + [ctypes.c_size_t] * 3
+                                      + [ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
+                                         ctypes.c_size_t, ctypes.c_void_p]),
     "b200_gemm_last_status": (ctypes.c_int, []),
     "b200_gemm_last_error": (ctypes.c_char_p, []),
     "b200_gemm_version": (ctypes.c_char_p, []),
@@ -243,6 +264,146 @@ class loader:
         t = self._type_index(C, A, types)
         _check(self._lib.b200_gemm_host(t, _ptr(C), _ptr(A), _ptr(B), M, N, K, batch_count,
                                         int(layout_c), int(layout_a), int(layout_b)))
+
+    # ---- products with epilogues, grouped products, gradients ------------------------------
+    def _place(self, stream, tensors, roles):
+        """Stream cell for a call on `tensors`, and the device to make current (None: already is).
+
+        Tensors must share one CUDA device, be dense (contiguous; every shape is given by the
+        sizes of the call) and be at least as long as the call needs; raw addresses are taken as
+        they are.  The call runs on the tensors' device and, where no stream is given, on that
+        device's current stream."""
+        device = None
+        for (name, size, kind), t in zip(roles, tensors):
+            if t is None or isinstance(t, int):
+                continue
+            if not t.is_cuda or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous CUDA tensor")
+            if device is None:
+                device = t.device
+            elif t.device != device:
+                raise ValueError(f"{name} is on {t.device}, other arguments on {device}")
+            if t.numel() < size:
+                raise ValueError(f"{name} holds {t.numel()} elements, the call needs {size}")
+            if kind is not None and t.dtype != kind:
+                raise ValueError(f"{name} is {t.dtype}, not {kind}")
+        if device is None:
+            return self._stream_ptr(stream), None
+        import torch
+        if stream is None:
+            stream = torch.cuda.current_stream(device)
+        elif getattr(stream, "device", device) != device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        return self._stream_ptr(stream), (device if device.index != torch.cuda.current_device() else None)
+
+    @staticmethod
+    def _on(device, call, *args) -> None:
+        if device is None:
+            st = call(*args)
+        else:
+            import torch
+            with torch.cuda.device(device):
+                st = call(*args)
+        if st != 0:
+            _check(st)
+
+    @staticmethod
+    def _epilogue(activation, gradient, bias, residual, preact, bias_grad, bias_stride):
+        act = ACTIVATIONS.get(activation, activation)
+        if not isinstance(act, int):
+            raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
+        return Epilogue(act, int(gradient), _ptr(bias), _ptr(residual), _ptr(preact), _ptr(bias_grad), bias_stride)
+
+    @staticmethod
+    def _f32(*tensors):
+        """torch.float32 if any of `tensors` is a tensor (else torch is not needed)."""
+        if all(t is None or isinstance(t, int) for t in tensors):
+            return None
+        import torch
+        return torch.float32
+
+    def gemm_fused(self, C, A, B, M, N, K, layout_c=0, layout_a=0, layout_b=0, batch_count=1, activation="none",
+                   bias=None, residual=None, preact=None, gradient=False, bias_grad=None, bias_stride=0,
+                   stream=None, types=None) -> None:
+        """`b200_gemm_fused`: a product and what a layer does around it, in one kernel.
+
+        Forward: `C = act(A*B + bias) + residual`; with `preact` given it receives `A*B + bias`.
+        `gradient=True`: `C = (A*B) * act'(preact)`, and `bias_grad` (float32) receives the column
+        sums of C.  `activation` is one of `ACTIVATIONS`; bias, residual and preact have C's type,
+        residual and preact C's layout; residual (forward) or preact (gradient) may be C itself.
+        With batch_count > 1, `bias_stride` 0 shares one bias among the items (its gradient is
+        the sum over them), N or more gives each its own."""
+        t = self._type_index(C, A, types)
+        mn, vec = batch_count * M * N, N + (batch_count - 1) * bias_stride if N else 0
+        ct = getattr(C, "dtype", None)
+        sp, dev = self._place(stream, (C, A, B, bias, residual, preact, bias_grad), (
+            ("C", mn, None), ("A", batch_count * M * K, None), ("B", batch_count * K * N, getattr(A, "dtype", None)),
+            ("bias", vec, ct), ("residual", mn, ct), ("preact", mn, ct), ("bias_grad", vec, self._f32(bias_grad))))
+        epi = self._epilogue(activation, gradient, bias, residual, preact, bias_grad, bias_stride)
+        self._on(dev, self._lib.b200_gemm_fused, t, _ptr(C), _ptr(A), _ptr(B), M, N, K, batch_count, int(layout_c),
+                 int(layout_a), int(layout_b), sp, ctypes.byref(epi))
+
+    def gemm_grouped(self, C, A, B, offsets, rows, N, K, groups, layout_b=0, activation="none", bias=None,
+                     residual=None, preact=None, gradient=False, bias_grad=None, stream=None, types=None) -> None:
+        """`b200_gemm_grouped`: rows [offsets[e], offsets[e+1]) of A (rows x K) times matrix e of B
+        (groups x K x N, each in layout_b), with the epilogues of `gemm_fused`.  `offsets` is an
+        int32 tensor of groups + 1 on the device; rows outside [offsets[0], offsets[groups]) are
+        left as they are.  bias and bias_grad are groups x N.  The input gradient is the same call
+        on the output's gradient with layout_b flipped and N and K exchanged."""
+        t = self._type_index(C, A, types)
+        mn, ct = rows * N, getattr(C, "dtype", None)
+        sp, dev = self._place(stream, (C, A, B, bias, residual, preact, bias_grad, offsets), (
+            ("C", mn, None), ("A", rows * K, None), ("B", groups * K * N, getattr(A, "dtype", None)),
+            ("bias", groups * N, ct), ("residual", mn, ct), ("preact", mn, ct),
+            ("bias_grad", groups * N, self._f32(bias_grad)), ("offsets", groups + 1, self._int32(offsets))))
+        epi = self._epilogue(activation, gradient, bias, residual, preact, bias_grad, 0)
+        self._on(dev, self._lib.b200_gemm_grouped, t, _ptr(C), _ptr(A), _ptr(B), _ptr(offsets), rows, N, K, groups,
+                 int(layout_b), sp, ctypes.byref(epi))
+
+    @staticmethod
+    def _int32(t):
+        if t is None or isinstance(t, int):
+            return None
+        import torch
+        return torch.int32
+
+    def gemm_grouped_wgrad(self, C, A, B, offsets, rows, M, N, groups, layout_c=0, accumulate=False, stream=None,
+                           types=None) -> None:
+        """`b200_gemm_grouped_wgrad`: for every group `C_e = A[rows of e]^T * B[rows of e]` (added to
+        C_e with `accumulate`), A rows x M, B rows x N, C groups x M x N, each C_e in layout_c.
+        An empty group's C_e is zero."""
+        t = self._type_index(C, A, types)
+        sp, dev = self._place(stream, (C, A, B, offsets), (
+            ("C", groups * M * N, None), ("A", rows * M, None), ("B", rows * N, getattr(A, "dtype", None)),
+            ("offsets", groups + 1, self._int32(offsets))))
+        self._on(dev, self._lib.b200_gemm_grouped_wgrad, t, _ptr(C), _ptr(A), _ptr(B), _ptr(offsets), rows, M, N,
+                 groups, int(layout_c), int(accumulate), sp)
+
+    _OUT_TYPES = None  # torch dtype of C -> a type pair with that output
+
+    def activation_backward(self, dZ, dY, preact, M, N, layout=0, batch_count=1, activation="none", bias_grad=None,
+                            bias_stride=0, offsets=None, groups=0, stream=None, types=None) -> None:
+        """`b200_gemm_activation_backward`: `dZ = dY * act'(preact)` and `bias_grad` (float32), the
+        column sums of dZ, for M x N matrices.  dZ may be None (only the sums), dY or preact
+        itself.  With `offsets` (int32 on the device, `groups` + 1) the rows are those of
+        `gemm_grouped` and bias_grad is groups x N."""
+        if types is None:
+            if loader._OUT_TYPES is None:
+                import torch
+                loader._OUT_TYPES = {torch.float16: 0, torch.float32: 3, torch.bfloat16: 2}
+            t = loader._OUT_TYPES[dY.dtype]
+        else:
+            t = TYPE_PAIRS[types] if isinstance(types, tuple) else int(types)
+        mn, ct = batch_count * M * N, getattr(dY, "dtype", None)
+        vec = groups * N if groups else (N + (batch_count - 1) * bias_stride if N else 0)
+        sp, dev = self._place(stream, (dZ, dY, preact, bias_grad, offsets), (
+            ("dZ", mn, ct), ("dY", mn, None), ("preact", mn, ct), ("bias_grad", vec, self._f32(bias_grad)),
+            ("offsets", groups + 1, self._int32(offsets))))
+        act = ACTIVATIONS.get(activation, activation)
+        if not isinstance(act, int):
+            raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
+        self._on(dev, self._lib.b200_gemm_activation_backward, t, _ptr(dZ), _ptr(dY), _ptr(preact), M, N, batch_count,
+                 int(layout), act, _ptr(bias_grad), bias_stride, _ptr(offsets), groups, sp)
 
 
 def get_gemm_params(m: int, n: int, k: int, layout_c=0, layout_a=0, layout_b=0, type_group: int = 0):

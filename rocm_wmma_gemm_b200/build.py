@@ -25,6 +25,8 @@ DEPENDS = SOURCES + [
     os.path.join(PKG_DIR, "csrc", "ptx_sm100.cuh"),
     os.path.join(PKG_DIR, "csrc", "config_table.inc"),
     os.path.join(PKG_DIR, "csrc", "slab_driver.inc"),
+    os.path.join(PKG_DIR, "csrc", "epilogue.cuh"),
+    os.path.join(PKG_DIR, "csrc", "epilogue_driver.inc"),
     os.path.join(ROOT_DIR, "include", "b200_gemm.h"),
 ]
 
@@ -33,6 +35,7 @@ NVCC_FLAGS = [
     "-lineinfo", "-O3", "-std=c++17",
     "-shared", "-Xcompiler", "-fPIC",
     "-diag-suppress", "177",
+    "-split-compile", "0",  # the kernels of one file are compiled on all cores
 ]
 
 

@@ -1,0 +1,500 @@
+// Device side of the products with epilogues and of the grouped products: the activation
+// functions and their derivatives, the epilogue's parameters, ragged-row bookkeeping, and the
+// kernels around the tcgen05 GEMM (CUDA-core product for operands TMA cannot address, bias
+// gradient sums, backward of an activation).
+//
+//   forward    Z = A*B + bias      C = act(Z) + residual          (Z kept on request)
+//   gradient   C = (A*B) .* act'(Z)      bias_grad = sum of C over the rows, before rounding
+//
+// All of it is computed in f32 from the f32 accumulators and rounded once, when C (and Z) are
+// stored; the bias gradient is a sum of the unrounded f32 values.
+#pragma once
+
+#include "ptx_sm100.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace b200 {
+
+// Activations.  silu and the tanh form of gelu are one function, x * sigmoid(x * (c0 + c1 x^2)):
+// silu has c0 = 1, c1 = 0; 0.5 x (1 + tanh(u)) = x * sigmoid(2 u) with
+// 2 u = 2 sqrt(2 / pi) (x + 0.044715 x^3).
+enum : uint32_t { ACT_NONE = 0, ACT_RELU = 1, ACT_SIGMOID = 2, ACT_GELU = 3 };
+
+enum : uint32_t { RAGGED_NONE = 0, RAGGED_ROWS = 1, RAGGED_K = 2 };
+
+constexpr uint32_t MAX_GROUPS = 1024;
+
+struct EpilogueParams {
+    const void*    bias;        // forward: nullptr or one value per column of the caller's C, C's type
+    const void*    residual;    // forward: nullptr or a matrix like C (may be C itself)
+    void*          preact;      // forward: nullptr or where Z goes; gradient: Z (may be C itself)
+    float*         part;        // gradient: nullptr or partial bias gradients [batch][part_blocks][length]
+    uint64_t       bias_stride; // elements between the biases of consecutive batch items / groups
+    uint32_t       act;
+    float          c0, c1;      // ACT_SIGMOID
+    uint32_t       gradient;
+    uint32_t       part_blocks; // blocks per batch item (all groups together)
+    uint32_t       part_rows;   // rows of the caller's C per block
+    uint32_t       ragged;
+    const int32_t* offsets;     // ragged: groups + 1 row offsets on the device
+    uint32_t       groups;
+    uint32_t       rows;        // ragged: rows of the ragged operands
+};
+
+// sigmoid in f32: e^-s overflows to infinity and its reciprocal to 0 far left, which is right.
+__device__ __forceinline__ float sigmoid_f32(float s) { return __fdividef(1.f, 1.f + __expf(-s)); }
+
+// (a NaN stays a NaN under every activation)
+template <uint32_t ACT>
+__device__ __forceinline__ float act_value(float x, float c0, float c1)
+{
+    if constexpr (ACT == ACT_RELU) return x < 0.f ? 0.f : x;
+    else if constexpr (ACT == ACT_SIGMOID) return x * sigmoid_f32(x * fmaf(c1 * x, x, c0));
+    else if constexpr (ACT == ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678f));
+    else return x;
+}
+
+template <uint32_t ACT>
+__device__ __forceinline__ float act_slope(float x, float c0, float c1)
+{
+    if constexpr (ACT == ACT_RELU) return x > 0.f ? 1.f : (x <= 0.f ? 0.f : x);
+    else if constexpr (ACT == ACT_SIGMOID) {
+        // d/dx x s(u(x)) = s + x s (1 - s) u'(x),  u = c0 x + c1 x^3
+        const float x2 = x * x;
+        const float s  = sigmoid_f32(x * fmaf(c1, x2, c0));
+        return fmaf(x * s * (1.f - s), fmaf(3.f * c1, x2, c0), s);
+    } else if constexpr (ACT == ACT_GELU) {
+        return fmaf(x * 0.39894228f, __expf(-0.5f * x * x), 0.5f * (1.f + erff(x * 0.70710678f)));
+    } else return 1.f;
+}
+
+// Calls f with the activation as a compile-time constant (the loop over a tile's elements is
+// inside f, so the choice is made once per chunk).
+template <uint32_t V>
+struct ActTag {
+    static constexpr uint32_t value = V;
+};
+template <class F>
+__device__ __forceinline__ void with_act(uint32_t act, F&& f)
+{
+    switch (act) {
+        case ACT_RELU: f(ActTag<ACT_RELU>{}); break;
+        case ACT_SIGMOID: f(ActTag<ACT_SIGMOID>{}); break;
+        case ACT_GELU: f(ActTag<ACT_GELU>{}); break;
+        default: f(ActTag<ACT_NONE>{}); break;
+    }
+}
+
+template <class T>
+__device__ __forceinline__ float to_f32(T v) { return static_cast<float>(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v)
+{
+    if constexpr (sizeof(T) == 4) return v;
+    else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+    else return __float2bfloat16_rn(v);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Ragged rows.  Group e owns rows [first_row(e), first_row(e + 1)).  Offsets are used as their
+// running maximum clamped to [0, rows]: whatever the array holds, every row index stays inside
+// the matrices, every row has at most one owner and the tiles of all groups together are at
+// most rows / tile + groups.
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t clamp_offset(int32_t v, uint32_t rows)
+{
+    return v < 0 ? 0u : min(static_cast<uint32_t>(v), rows);
+}
+
+__device__ __forceinline__ uint32_t warp_scan_max(uint32_t v, uint32_t lane)
+{
+#pragma unroll
+    for (uint32_t d = 1; d < 32; d *= 2) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v = max(v, t);
+    }
+    return v;
+}
+
+__device__ __forceinline__ uint32_t warp_scan_add(uint32_t v, uint32_t lane)
+{
+#pragma unroll
+    for (uint32_t d = 1; d < 32; d *= 2) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += t;
+    }
+    return v;
+}
+
+// First partial-sum block of a group: blocks of `part_rows` rows start at the group's first row.
+// floor(first / b) + e is non-decreasing and leaves room for ceil(length / b) blocks per group.
+__device__ __forceinline__ uint32_t group_first_block(uint32_t first_row, uint32_t e, uint32_t part_rows)
+{
+    return first_row / part_rows + e;
+}
+
+// The group and rows of row-tile number `want` (tiles of `tile` rows, groups in order); the whole
+// warp takes part.  False when there are fewer tiles.
+__device__ __forceinline__ bool locate_row_tile(const int32_t* __restrict__ offsets, uint32_t groups, uint32_t rows,
+                                                uint32_t tile, uint32_t want, uint32_t& e, uint32_t& first,
+                                                uint32_t& row0, uint32_t& row1)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t       top = 0u, before = 0u; // running maximum of the offsets, tiles of the groups so far
+    for (uint32_t g0 = 0; g0 < groups; g0 += 32u) {
+        const uint32_t g  = g0 + lane;
+        uint32_t       lo = g < groups ? clamp_offset(__ldg(offsets + g), rows) : 0u;
+        uint32_t       hi = g < groups ? clamp_offset(__ldg(offsets + g + 1u), rows) : 0u;
+        lo = max(warp_scan_max(lo, lane), top);
+        hi = max(warp_scan_max(hi, lane), lo);
+        const uint32_t tiles = g < groups ? (hi - lo + tile - 1u) / tile : 0u;
+        const uint32_t incl  = before + warp_scan_add(tiles, lane);
+        const uint32_t hit   = __ballot_sync(0xffffffffu, want < incl);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            e             = g0 + src;
+            first         = __shfl_sync(0xffffffffu, lo, src);
+            const uint32_t end = __shfl_sync(0xffffffffu, hi, src);
+            const uint32_t tb  = __shfl_sync(0xffffffffu, incl - tiles, src);
+            row0               = first + (want - tb) * tile;
+            row1               = min(end, row0 + tile);
+            return true;
+        }
+        top    = __shfl_sync(0xffffffffu, hi, 31);
+        before = __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return false;
+}
+
+// Rows [lo, hi) of group e; the whole warp takes part.
+__device__ __forceinline__ void group_rows(const int32_t* __restrict__ offsets, uint32_t e, uint32_t rows, uint32_t& lo,
+                                           uint32_t& hi)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t       top  = 0u;
+    for (uint32_t g = lane; g <= e; g += 32u) top = max(top, clamp_offset(__ldg(offsets + g), rows));
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+    lo = top;
+    hi = max(lo, clamp_offset(__ldg(offsets + e + 1u), rows));
+}
+
+// ---------------------------------------------------------------------------------------------
+// CUDA-core product with epilogue, arbitrary element strides, f32 accumulation in ascending k:
+// a 64 x 64 tile of C per block, 4 x 4 elements per thread.  Serves what TMA cannot address
+// (a contiguous extent that is not a multiple of 16 bytes).  One kernel for the dense, the
+// grouped (ragged rows) and the weight-gradient (ragged K) products.
+// ---------------------------------------------------------------------------------------------
+struct SimpleParams {
+    const void* A;
+    const void* B;
+    void*       C;
+    uint32_t    M, N, K;
+    uint32_t    n_tiles;
+    uint64_t    a_sm, a_sk, b_sk, b_sn, c_sm, c_sn; // element strides
+    uint64_t    a_sb, b_sb, c_sb;                   // per batch item / group
+    uint32_t    z0;                                 // first batch item of this launch
+};
+
+constexpr uint32_t SIMPLE_TILE = 64;
+
+template <class TIn, class TOut>
+__global__ void __launch_bounds__(256) simple_product_kernel(const SimpleParams p, const EpilogueParams ep)
+{
+    __shared__ float    sA[16][SIMPLE_TILE + 4];
+    __shared__ float    sB[16][SIMPLE_TILE + 4];
+    __shared__ uint32_t s_where[4];
+    const uint32_t tid = threadIdx.x, tx = tid & 15u, ty = tid >> 4;
+    const uint32_t j0  = (blockIdx.x % p.n_tiles) * SIMPLE_TILE;
+    const uint32_t mt  = blockIdx.x / p.n_tiles;
+    uint32_t       z = blockIdx.z + p.z0, m0 = mt * SIMPLE_TILE, m1 = min(p.M, m0 + SIMPLE_TILE), k0 = 0u, k1 = p.K, first = 0u;
+    if (ep.ragged == RAGGED_ROWS) {
+        if (tid < 32u) {
+            uint32_t   e = 0, f = 0, r0 = 0, r1 = 0;
+            const bool ok = locate_row_tile(ep.offsets, ep.groups, ep.rows, SIMPLE_TILE, mt, e, f, r0, r1);
+            if (tid == 0) {
+                s_where[0] = ok ? e : 0xffffffffu;
+                s_where[1] = r0;
+                s_where[2] = r1;
+                s_where[3] = f;
+            }
+        }
+        __syncthreads();
+        z = s_where[0];
+        if (z == 0xffffffffu) return; // (the whole block)
+        m0    = s_where[1];
+        m1    = s_where[2];
+        first = s_where[3];
+    } else if (ep.ragged == RAGGED_K) {
+        if (tid < 32u) {
+            uint32_t lo, hi;
+            group_rows(ep.offsets, z, ep.rows, lo, hi);
+            if (tid == 0) {
+                s_where[0] = lo;
+                s_where[1] = hi;
+            }
+        }
+        __syncthreads();
+        k0 = s_where[0];
+        k1 = s_where[1];
+    }
+    // ragged rows: A and C are addressed by global row; ragged K: A and B by global row of the sum
+    const TIn* A = static_cast<const TIn*>(p.A) + (ep.ragged == RAGGED_NONE ? z * p.a_sb : 0u);
+    const TIn* B = static_cast<const TIn*>(p.B) + (ep.ragged != RAGGED_K ? z * p.b_sb : 0u);
+    const uint64_t c_base = ep.ragged != RAGGED_ROWS ? z * p.c_sb : 0u;
+
+    float acc[4][4] = {};
+    for (uint32_t k = k0; k < k1; k += 16u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // neighbouring threads read along whichever index is contiguous
+            const uint32_t ka = p.a_sk == 1 ? tx : ty, ma = (p.a_sk == 1 ? ty : tx) + 16u * i;
+            sA[ka][ma] = (k + ka < k1 && m0 + ma < m1) ? to_f32(A[(m0 + ma) * p.a_sm + (k + ka) * p.a_sk]) : 0.f;
+            const uint32_t kb = p.b_sk == 1 ? tx : ty, nb = (p.b_sk == 1 ? ty : tx) + 16u * i;
+            sB[kb][nb] = (k + kb < k1 && j0 + nb < p.N) ? to_f32(B[(k + kb) * p.b_sk + (j0 + nb) * p.b_sn]) : 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int kk = 0; kk < 16; ++kk) {
+            float a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = sA[kk][ty + 16 * i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = sB[kk][tx + 16 * j];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        }
+        __syncthreads();
+    }
+    TOut*       C    = static_cast<TOut*>(p.C) + c_base;
+    const TOut* bias = static_cast<const TOut*>(ep.bias);
+    const TOut* res  = ep.residual ? static_cast<const TOut*>(ep.residual) + c_base : nullptr;
+    TOut*       pre  = ep.preact ? static_cast<TOut*>(ep.preact) + c_base : nullptr;
+    with_act(ep.act, [&](auto tag) {
+        constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t m = m0 + ty + 16u * i, n = j0 + tx + 16u * j;
+                if (m < m1 && n < p.N) {
+                    const uint64_t at = m * p.c_sm + n * p.c_sn;
+                    float          v  = acc[i][j];
+                    if (ep.gradient) {
+                        if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(pre[at]), ep.c0, ep.c1));
+                    } else {
+                        if (bias) v += to_f32(bias[z * ep.bias_stride + n]);
+                        if (pre) pre[at] = from_f32<TOut>(v);
+                        v = act_value<ACT>(v, ep.c0, ep.c1);
+                        if (res) v += to_f32(res[at]);
+                    }
+                    C[at]     = from_f32<TOut>(v);
+                    acc[i][j] = v;
+                } else {
+                    acc[i][j] = 0.f;
+                }
+            }
+        }
+    });
+    if (ep.part) { // column sums of the tile, rows in a fixed order
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sA[ty][tx + 16 * j] = (acc[0][j] + acc[1][j]) + (acc[2][j] + acc[3][j]);
+        __syncthreads();
+        if (tid < SIMPLE_TILE && j0 + tid < p.N) {
+            float s = 0.f;
+            for (int i = 0; i < 16; ++i) s += sA[i][tid];
+            const uint64_t block = ep.ragged == RAGGED_ROWS
+                                       ? group_first_block(first, z, SIMPLE_TILE) + (m0 - first) / SIMPLE_TILE
+                                       : static_cast<uint64_t>(z) * ep.part_blocks + mt;
+            ep.part[block * p.N + j0 + tid] = s;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Bias gradient from the partial sums: out[g][n] = sum over g's blocks of part[block][n], blocks
+// in a fixed order, so the result does not depend on timing.  blockIdx.y = g: a batch item
+// (`items` items per output: all of them when the bias is shared) or a group of ragged rows.
+// ---------------------------------------------------------------------------------------------
+constexpr uint32_t SUM_LANES = 16;
+
+__global__ void __launch_bounds__(32 * SUM_LANES)
+    bias_grad_sum_kernel(const float* __restrict__ part, float* __restrict__ out, uint32_t length, uint64_t out_stride,
+                         uint64_t blocks, const int32_t* __restrict__ offsets, uint32_t rows, uint32_t part_rows)
+{
+    __shared__ float s_sum[SUM_LANES][32];
+    const uint32_t tx = threadIdx.x & 31u, ty = threadIdx.x >> 5, n = blockIdx.x * 32u + tx;
+    ptx::grid_dep_wait(); // the partial sums are those of the kernel before this one
+    ptx::grid_dep_launch();
+    uint64_t b0 = static_cast<uint64_t>(blockIdx.y) * blocks, count = blocks;
+    if (offsets) {
+        uint32_t lo, hi;
+        group_rows(offsets, blockIdx.y, rows, lo, hi);
+        b0    = group_first_block(lo, blockIdx.y, part_rows);
+        count = (hi - lo + part_rows - 1u) / part_rows;
+    }
+    float s = 0.f;
+    if (n < length)
+#pragma unroll 4
+        for (uint64_t b = ty; b < count; b += SUM_LANES) s += __ldg(part + (b0 + b) * length + n);
+    s_sum[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && n < length) {
+        float t = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < SUM_LANES; ++i) t += s_sum[i][tx];
+        out[blockIdx.y * out_stride + n] = t;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Backward of an activation where no product precedes it: dZ = dY .* act'(Z), and the sums of dZ
+// over the rows (of the rounded f32 products: no contraction into the sum, so that the sums are the
+// same bits whether dZ is stored or not).  Memory view: `lines` lines of `length` contiguous elements.  Row-major C: a
+// line is a row and the sums run over lines; column-major C: a line is a column and the sums run
+// along it.
+// ---------------------------------------------------------------------------------------------
+struct ActBackwardParams {
+    void*       dz;     // nullptr: only the sums are wanted
+    const void* dy;
+    const void* z;      // nullptr with ACT_NONE
+    uint32_t    lines, length;
+    uint32_t    strip;  // row-major: lines per block; column-major: elements of a line per block
+    uint32_t    blocks_x;
+    uint64_t    stride; // elements per batch item
+    uint32_t    z0;
+};
+
+// 16 bytes of T.
+template <class T>
+struct Pack {
+    static constexpr int N = 16 / sizeof(T);
+    uint4                raw;
+    __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(&raw)[i]); }
+    __device__ __forceinline__ void  set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f32<T>(v); }
+};
+
+// Row-major: each thread owns V consecutive columns (V = 16 bytes' worth, or 1 where the rows are
+// not 16-byte aligned) and walks the strip's lines; threads of equal column and different
+// threadIdx.y share a strip and add their sums through shared memory.
+template <class T, int V>
+__global__ void __launch_bounds__(256) act_backward_rows_kernel(const ActBackwardParams p, const EpilogueParams ep)
+{
+    __shared__ float    s_sum[256 * V];
+    __shared__ uint32_t s_where[4];
+    const uint32_t tx = threadIdx.x, ty = threadIdx.y, tid = ty * blockDim.x + tx;
+    const uint32_t n  = ((blockIdx.x % p.blocks_x) * blockDim.x + tx) * V;
+    const uint32_t st = blockIdx.x / p.blocks_x;
+    uint32_t       r0 = st * p.strip, r1 = min(p.lines, r0 + p.strip);
+    uint64_t       block = static_cast<uint64_t>(blockIdx.z + p.z0) * ep.part_blocks + st;
+    if (ep.ragged == RAGGED_ROWS) {
+        if (tid < 32u) {
+            uint32_t   e = 0, first = 0, a = 0, b = 0;
+            const bool ok = locate_row_tile(ep.offsets, ep.groups, ep.rows, p.strip, st, e, first, a, b);
+            if (tid == 0) {
+                s_where[0] = ok ? 1u : 0u;
+                s_where[1] = a;
+                s_where[2] = b;
+                s_where[3] = group_first_block(first, e, p.strip) + (a - first) / p.strip;
+            }
+        }
+        __syncthreads();
+        if (!s_where[0]) return;
+        r0    = s_where[1];
+        r1    = s_where[2];
+        block = s_where[3];
+    }
+    const uint64_t base = (blockIdx.z + p.z0) * p.stride;
+    const T*       dy   = static_cast<const T*>(p.dy) + base;
+    const T*       z    = p.z ? static_cast<const T*>(p.z) + base : nullptr;
+    T*             dz   = p.dz ? static_cast<T*>(p.dz) + base : nullptr;
+    float          sum[V] = {};
+    if (n < p.length) {
+        with_act(ep.act, [&](auto tag) {
+            constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll 4
+            for (uint32_t r = r0 + ty; r < r1; r += blockDim.y) {
+                const uint64_t at = static_cast<uint64_t>(r) * p.length + n;
+                if constexpr (V > 1) {
+                    Pack<T> g, x, o;
+                    g.raw = __ldcs(reinterpret_cast<const uint4*>(dy + at));
+                    if (ACT != ACT_NONE) x.raw = __ldcs(reinterpret_cast<const uint4*>(z + at));
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        float v = g.get(i);
+                        if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(x.get(i), ep.c0, ep.c1));
+                        o.set(i, v);
+                        sum[i] += v;
+                    }
+                    if (dz) *reinterpret_cast<uint4*>(dz + at) = o.raw;
+                } else {
+                    float v = to_f32(dy[at]);
+                    if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(z[at]), ep.c0, ep.c1));
+                    if (dz) dz[at] = from_f32<T>(v);
+                    sum[0] += v;
+                }
+            }
+        });
+    }
+    if (!ep.part) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) s_sum[tid * V + i] = sum[i];
+    __syncthreads();
+    if (ty == 0 && n < p.length) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float t = 0.f;
+            for (uint32_t y = 0; y < blockDim.y; ++y) t += s_sum[(y * blockDim.x + tx) * V + i];
+            ep.part[block * p.length + n + i] = t;
+        }
+    }
+}
+
+// Column-major: one warp per line and strip.
+template <class T, int V>
+__global__ void __launch_bounds__(256) act_backward_cols_kernel(const ActBackwardParams p, const EpilogueParams ep)
+{
+    const uint32_t lane = threadIdx.x, line = (blockIdx.x / p.blocks_x) * blockDim.y + threadIdx.y;
+    const uint32_t st = blockIdx.x % p.blocks_x;
+    if (line >= p.lines) return;
+    const uint32_t e0 = st * p.strip, e1 = min(p.length, e0 + p.strip);
+    const uint64_t base = (blockIdx.z + p.z0) * p.stride + static_cast<uint64_t>(line) * p.length;
+    const T*       dy   = static_cast<const T*>(p.dy) + base;
+    const T*       z    = p.z ? static_cast<const T*>(p.z) + base : nullptr;
+    T*             dz   = p.dz ? static_cast<T*>(p.dz) + base : nullptr;
+    float          sum  = 0.f;
+    with_act(ep.act, [&](auto tag) {
+        constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll 4
+        for (uint32_t i0 = e0 + lane * V; i0 < e1; i0 += 32u * V) {
+            if constexpr (V > 1) {
+                Pack<T> g, x, o;
+                g.raw = __ldcs(reinterpret_cast<const uint4*>(dy + i0));
+                if (ACT != ACT_NONE) x.raw = __ldcs(reinterpret_cast<const uint4*>(z + i0));
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float v = g.get(i);
+                    if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(x.get(i), ep.c0, ep.c1));
+                    o.set(i, v);
+                    sum += v;
+                }
+                if (dz) *reinterpret_cast<uint4*>(dz + i0) = o.raw;
+            } else {
+                float v = to_f32(dy[i0]);
+                if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(z[i0]), ep.c0, ep.c1));
+                if (dz) dz[i0] = from_f32<T>(v);
+                sum += v;
+            }
+        }
+    });
+    if (!ep.part) return;
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) ep.part[(static_cast<uint64_t>(blockIdx.z + p.z0) * ep.part_blocks + st) * p.lines + line] = sum;
+}
+
+} // namespace b200

@@ -7,6 +7,7 @@
 // There is no CPU fallback: without a CUDA device every compute entry point fails.
 #include "../../include/b200_gemm.h"
 #include "gemm_kernels.cuh"
+#include "epilogue.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -158,6 +159,8 @@ struct PairCache {
     uint32_t smem[3]  = {0, 0, 0};
 };
 
+enum : int { WS_SPLIT_K = 0, WS_EPILOGUE = 1 };
+
 struct DeviceCtx {
     std::atomic<bool> ready{false}; // set last, read first: initialised contexts skip the lock
     int           sm_count = 0;
@@ -170,6 +173,7 @@ struct DeviceCtx {
         cudaStream_t stream;
         float*       ptr;
         size_t       bytes;
+        int          kind; // WS_SPLIT_K or WS_EPILOGUE: a call may use one of each
     };
     std::vector<Workspace> workspaces;
     // buffers a workspace has outgrown: freed once the work that was queued on them has drained
@@ -307,7 +311,7 @@ static int get_ctx(DeviceCtx** out)
 // the steady state allocates nothing (an allocation per call costs more than a skinny GEMM).
 // A buffer that has become too small is not freed here - kernels queued on the stream may still
 // use it - but retired behind an event and freed by a later call once that event has passed.
-static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, float** out)
+static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, float** out, int kind = WS_SPLIT_K)
 {
     std::lock_guard<std::mutex> lock(ctx->ws_mutex);
     for (size_t i = 0; i < ctx->retired.size();) {
@@ -322,7 +326,7 @@ static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, floa
         }
     }
     for (auto& w : ctx->workspaces) {
-        if (w.stream != stream) continue;
+        if (w.stream != stream || w.kind != kind) continue;
         if (w.bytes < bytes) {
             const size_t want  = bytes + bytes / 4;
             float*       fresh = nullptr;
@@ -343,7 +347,7 @@ static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, floa
         *out = w.ptr;
         return B200_GEMM_OK;
     }
-    DeviceCtx::Workspace w{stream, nullptr, 0};
+    DeviceCtx::Workspace w{stream, nullptr, 0, kind};
     CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&w.ptr), bytes));
     w.bytes = bytes;
     ctx->workspaces.push_back(w);
@@ -1850,3 +1854,4 @@ extern "C" int b200_gemm_debug_cta_times(unsigned long long* cta)
 #endif
 
 #include "slab_driver.inc"
+#include "epilogue_driver.inc"
