@@ -10,6 +10,7 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT_DIR = os.path.dirname(PKG_DIR)
@@ -19,13 +20,14 @@ LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 # every launch (see csrc/gemm_kernels.cuh and timeline.py).  A profiling build, never loaded by
 # the package itself.
 TIMELINE_LIB_PATH = os.path.join(PKG_DIR, "librocm_wmma_gemm_sm100a_timeline.so")
-SOURCES = [os.path.join(PKG_DIR, "csrc", "gemm_lib.cu")]
+SOURCES = [os.path.join(PKG_DIR, "csrc", "gemm_lib.cu"), os.path.join(PKG_DIR, "csrc", "epilogue_kernels.cu")]
 DEPENDS = SOURCES + [
     os.path.join(PKG_DIR, "csrc", "gemm_kernels.cuh"),
     os.path.join(PKG_DIR, "csrc", "ptx_sm100.cuh"),
     os.path.join(PKG_DIR, "csrc", "config_table.inc"),
     os.path.join(PKG_DIR, "csrc", "slab_driver.inc"),
     os.path.join(PKG_DIR, "csrc", "epilogue.cuh"),
+    os.path.join(PKG_DIR, "csrc", "epilogue_kernels.cuh"),
     os.path.join(PKG_DIR, "csrc", "epilogue_driver.inc"),
     os.path.join(ROOT_DIR, "include", "b200_gemm.h"),
 ]
@@ -33,7 +35,7 @@ DEPENDS = SOURCES + [
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
     "-diag-suppress", "177",
     "-split-compile", "0",  # the kernels of one file are compiled on all cores
 ]
@@ -54,12 +56,23 @@ def is_stale(path: str = LIB_PATH) -> bool:
 
 
 def _compile(out: str, extra: list, verbose: bool) -> str:
-    cmd = [_nvcc()] + NVCC_FLAGS + extra + (["-Xptxas", "-v"] if verbose else []) + ["-o", out] + SOURCES + ["-ldl"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose:
-        sys.stderr.write(proc.stderr)
-    if proc.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + proc.stdout + proc.stderr)
+    # one object per source, compiled side by side, then linked
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, os.path.basename(src) + ".o") for src in SOURCES]
+        cmds = [[_nvcc()] + NVCC_FLAGS + extra + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", o, src]
+                for o, src in zip(objects, SOURCES)]
+        procs = [subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for cmd in cmds]
+        outputs = [p.communicate()[0] for p in procs]
+        cmds.append([_nvcc()] + NVCC_FLAGS[:2] + ["-shared", "-o", out] + objects + ["-ldl"])
+        if all(p.returncode == 0 for p in procs):
+            link = subprocess.run(cmds[-1], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+            procs.append(link)
+            outputs.append(link.stdout)
+        for cmd, proc, text in zip(cmds, procs, outputs):
+            if verbose:
+                sys.stderr.write(text)
+            if proc.returncode != 0:
+                raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + text)
     return out
 
 

@@ -15,6 +15,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace b200 {
 
 // Activations.  silu and the tanh form of gelu are one function, x * sigmoid(x * (c0 + c1 x^2)):
@@ -41,6 +43,13 @@ struct EpilogueParams {
     const int32_t* offsets;     // ragged: groups + 1 row offsets on the device
     uint32_t       groups;
     uint32_t       rows;        // ragged: rows of the ragged operands
+    // tcgen05 kernels only
+    uint32_t           bias_on_rows; // the bias runs along the kernel view's rows, not its columns
+    uint32_t           streamed;     // a matrix is read through the staging buffers (EpilogueMaps::in)
+    uint32_t           aux;          // Z is written (EpilogueMaps::aux)
+    uint32_t           bufs;         // staging buffers per warp for C: 1 or 2
+    uint32_t           table_at;     // ragged: byte offset of the group table in dynamic shared memory
+    const CUtensorMap* maps;         // ragged K: two maps per group, their row extents ending at the group's end
 };
 
 // sigmoid in f32: e^-s overflows to infinity and its reciprocal to 0 far left, which is right.
@@ -322,7 +331,7 @@ __global__ void __launch_bounds__(256) simple_product_kernel(const SimpleParams 
 // ---------------------------------------------------------------------------------------------
 constexpr uint32_t SUM_LANES = 16;
 
-__global__ void __launch_bounds__(32 * SUM_LANES)
+static __global__ void __launch_bounds__(32 * SUM_LANES)
     bias_grad_sum_kernel(const float* __restrict__ part, float* __restrict__ out, uint32_t length, uint64_t out_stride,
                          uint64_t blocks, const int32_t* __restrict__ offsets, uint32_t rows, uint32_t part_rows)
 {

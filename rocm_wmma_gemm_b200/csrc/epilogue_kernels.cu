@@ -1,0 +1,147 @@
+// The tcgen05 kernels with an epilogue: instantiations and launches.
+#include "epilogue_kernels.cuh"
+
+namespace b200 {
+
+namespace {
+
+template <class K>
+cudaError_t allow_smem(K kernel)
+{
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)EPI_SMEM_LIMIT);
+}
+
+template <int BN, int CL, bool TR, bool KS>
+cudaError_t set_one()
+{
+    cudaError_t e;
+    if constexpr (KS) {
+        e = allow_smem(gemm_epilogue_ksplit_kernel<BN, OUT_F32, TR>);
+        if (e == cudaSuccess) e = allow_smem(gemm_epilogue_ksplit_kernel<BN, OUT_F16, TR>);
+        if (e == cudaSuccess) e = allow_smem(gemm_epilogue_ksplit_kernel<BN, OUT_BF16, TR>);
+    } else {
+        e = allow_smem(gemm_epilogue_kernel<BN, OUT_F32, CL, TR>);
+        if (e == cudaSuccess) e = allow_smem(gemm_epilogue_kernel<BN, OUT_F16, CL, TR>);
+        if (e == cudaSuccess) e = allow_smem(gemm_epilogue_kernel<BN, OUT_BF16, CL, TR>);
+    }
+    return e;
+}
+
+template <int BN, int CL, bool TR, bool KS>
+cudaError_t launch_one(const EpilogueLaunch& l, cudaStream_t s)
+{
+    cudaLaunchConfig_t  lc = {};
+    const uint32_t      cluster = KS ? l.split : CL;
+    lc.gridDim          = dim3(l.units * cluster);
+    lc.blockDim         = dim3(EPI_THREADS);
+    lc.dynamicSmemBytes = l.smem;
+    lc.stream           = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id                                         = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x                           = cluster;
+    attr[0].val.clusterDim.y                           = 1;
+    attr[0].val.clusterDim.z                           = 1;
+    attr[1].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs                                           = attr;
+    lc.numAttrs                                        = 2;
+    auto go = [&](auto kernel) { return cudaLaunchKernelEx(&lc, kernel, l.a, l.b, l.d, l.em, l.gp, l.ep); };
+    if constexpr (KS) {
+        switch (l.out) {
+            case OUT_F32: return go(gemm_epilogue_ksplit_kernel<BN, OUT_F32, TR>);
+            case OUT_F16: return go(gemm_epilogue_ksplit_kernel<BN, OUT_F16, TR>);
+            default: return go(gemm_epilogue_ksplit_kernel<BN, OUT_BF16, TR>);
+        }
+    } else {
+        switch (l.out) {
+            case OUT_F32: return go(gemm_epilogue_kernel<BN, OUT_F32, CL, TR>);
+            case OUT_F16: return go(gemm_epilogue_kernel<BN, OUT_F16, CL, TR>);
+            default: return go(gemm_epilogue_kernel<BN, OUT_BF16, CL, TR>);
+        }
+    }
+}
+
+} // namespace
+
+cudaError_t set_epilogue_attributes()
+{
+    cudaError_t e = set_one<64, 1, false, false>();
+    if (e == cudaSuccess) e = set_one<128, 1, false, false>();
+    if (e == cudaSuccess) e = set_one<256, 1, false, false>();
+    if (e == cudaSuccess) e = set_one<256, 2, false, false>();
+    if (e == cudaSuccess) e = set_one<512, 2, false, false>();
+    if (e == cudaSuccess) e = set_one<16, 1, true, false>();
+    if (e == cudaSuccess) e = set_one<32, 1, true, false>();
+    if (e == cudaSuccess) e = set_one<64, 1, true, false>();
+    if (e == cudaSuccess) e = set_one<128, 1, true, false>();
+    if (e == cudaSuccess) e = set_one<128, 1, false, true>();
+    if (e == cudaSuccess) e = set_one<256, 1, false, true>();
+    if (e == cudaSuccess) e = set_one<16, 1, true, true>();
+    if (e == cudaSuccess) e = set_one<32, 1, true, true>();
+    if (e == cudaSuccess) e = set_one<64, 1, true, true>();
+    return e;
+}
+
+cudaError_t launch_epilogue_gemm(const EpilogueLaunch& l, cudaStream_t s)
+{
+    const bool ks = l.split > 1;
+    if (l.tr) {
+        switch (l.bn) {
+            case 16: return ks ? launch_one<16, 1, true, true>(l, s) : launch_one<16, 1, true, false>(l, s);
+            case 32: return ks ? launch_one<32, 1, true, true>(l, s) : launch_one<32, 1, true, false>(l, s);
+            case 64: return ks ? launch_one<64, 1, true, true>(l, s) : launch_one<64, 1, true, false>(l, s);
+            case 128: return ks ? cudaErrorInvalidValue : launch_one<128, 1, true, false>(l, s);
+        }
+    } else if (ks) {
+        switch (l.bn) {
+            case 128: return launch_one<128, 1, false, true>(l, s);
+            case 256: return launch_one<256, 1, false, true>(l, s);
+        }
+    } else if (l.cl == 2) {
+        switch (l.bn) {
+            case 256: return launch_one<256, 2, false, false>(l, s);
+            case 512: return launch_one<512, 2, false, false>(l, s);
+        }
+    } else {
+        switch (l.bn) {
+            case 64: return launch_one<64, 1, false, false>(l, s);
+            case 128: return launch_one<128, 1, false, false>(l, s);
+            case 256: return launch_one<256, 1, false, false>(l, s);
+        }
+    }
+    return cudaErrorInvalidValue; // not a compiled width
+}
+
+cudaError_t epilogue_pairs(int bn, uint32_t smem, int* pairs)
+{
+    cudaLaunchConfig_t q = {};
+    q.gridDim            = dim3(2 * 148);
+    q.blockDim           = dim3(EPI_THREADS);
+    q.dynamicSmemBytes   = smem;
+    cudaLaunchAttribute a[1];
+    a[0].id               = cudaLaunchAttributeClusterDimension;
+    a[0].val.clusterDim.x = 2;
+    a[0].val.clusterDim.y = 1;
+    a[0].val.clusterDim.z = 1;
+    q.attrs               = a;
+    q.numAttrs            = 1;
+    return bn == 512 ? cudaOccupancyMaxActiveClusters(pairs, gemm_epilogue_kernel<512, OUT_F32, 2>, &q)
+                     : cudaOccupancyMaxActiveClusters(pairs, gemm_epilogue_kernel<256, OUT_F32, 2>, &q);
+}
+
+cudaError_t launch_ragged_maps(const CUtensorMap& a, const CUtensorMap& b, CUtensorMap* maps, const int32_t* offsets, uint32_t groups,
+                               uint32_t rows, cudaStream_t s)
+{
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim            = dim3(groups);
+    lc.blockDim           = dim3(32);
+    lc.stream             = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs                                           = attr;
+    lc.numAttrs                                        = 1;
+    return cudaLaunchKernelEx(&lc, ragged_maps_kernel, a, b, maps, offsets, rows);
+}
+
+} // namespace b200

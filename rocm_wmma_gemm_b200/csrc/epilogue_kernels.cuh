@@ -1,0 +1,30 @@
+// Launch interface of the tcgen05 kernels with an epilogue.  They are compiled in a translation
+// unit of their own (epilogue_kernels.cu); the driver (epilogue_driver.inc) fills in a launch.
+#pragma once
+
+#include "gemm_kernels.cuh"
+
+namespace b200 {
+
+struct EpilogueLaunch {
+    int            bn;       // compiled tile width
+    int            cl;       // CTAs per tile
+    int            out;      // OUT_*
+    bool           tr;       // transposing epilogue
+    uint32_t       split;    // K partitions in a cluster (1: none)
+    uint32_t       units;    // CTAs, CTA pairs or clusters
+    uint32_t       smem;
+    CUtensorMap    a, b, d;
+    EpilogueMaps   em;
+    GemmParams     gp;
+    EpilogueParams ep;
+};
+
+cudaError_t set_epilogue_attributes();
+cudaError_t launch_epilogue_gemm(const EpilogueLaunch& l, cudaStream_t s);
+// CTA pairs of the kernel that can be resident at once.
+cudaError_t epilogue_pairs(int bn, uint32_t smem, int* pairs);
+cudaError_t launch_ragged_maps(const CUtensorMap& a, const CUtensorMap& b, CUtensorMap* maps, const int32_t* offsets, uint32_t groups,
+                               uint32_t rows, cudaStream_t s);
+
+} // namespace b200

@@ -12,6 +12,7 @@
 // (reference semantics: rocm_wmma_gemm/include/rocm_wmma_gemm/gemm.hpp:50-73).
 #pragma once
 
+#include "epilogue.cuh"
 #include "ptx_sm100.cuh"
 
 #include <type_traits>
@@ -125,9 +126,14 @@ constexpr int      UMMA_K         = 16;
 constexpr int      MAX_STAGES     = 12; // ring depth of the staged-epilogue kernels
 constexpr int      MAX_SLAB_STAGES = 24; // ring depth of the transposed-epilogue (slab) kernels
 constexpr int      GEMM_THREADS   = 192; // warp 0 TMA, warp 1 MMA, warps 2..5 epilogue
+constexpr int      EPI_WARPS      = 8;   // kernels with an epilogue (activation ...): warps 2..9, two per TMEM lane quarter
+constexpr int      EPI_THREADS    = 64 + 32 * EPI_WARPS;
 constexpr uint32_t A_TILE_BYTES   = BLOCK_M * BLOCK_K * 2;
 constexpr uint32_t EPI_BUF_BYTES  = 32 * 128; // one warp's 32 rows x 128 B
 constexpr uint32_t EPI_BYTES      = 4 * 2 * EPI_BUF_BYTES;
+// Dynamic shared memory a kernel with an epilogue may use: 227 KiB minus its static part (barriers
+// and biases, under 1.5 KiB).
+constexpr uint32_t EPI_SMEM_LIMIT = 232448u - 1536u;
 constexpr uint64_t WAIT_LIMIT_NS  = 2000000000ull; // 2 s per bounded wait
 
 // Bytes of one ring slot in one CTA: A' 128 x 64 plus B' (bn / cluster) x 64.
@@ -228,6 +234,11 @@ struct WorkCoord {
     uint32_t z_out;    // third TMA coordinate of D: batch * split_k + split
     uint32_t kb0, kb1; // k-block range
     uint32_t partial;  // balanced schedule: the segment is only part of its tile's K loop (f32 partial to the workspace)
+    // kernels with an epilogue only
+    uint32_t z_a, z_b; // third TMA coordinates of A' and B' (grouped products: 0, or the group)
+    uint32_t k_first;  // ragged K: first row of the group (0 otherwise)
+    uint32_t end;      // end of the ragged extent's group: rows (columns with the transposed epilogue) from here on are not ours
+    uint32_t group, first; // group, its first row
 };
 
 // Tile index -> (tile-row, tile-column) under the problem's raster.
@@ -371,6 +382,91 @@ __device__ __forceinline__ bool work_next(const GemmParams& p, WorkCursor& cur, 
     return true;
 }
 
+// ---------------------------------------------------------------------------------------------
+// Work of the kernels with an epilogue.  Dense problems: the plain schedule.  Ragged rows: the
+// groups' tiles one group after the other, within a group the ragged extent fastest, so that the
+// tiles in flight share the group's matrix; ragged K: every group has the same tiles, its K loop
+// runs over its own rows.  The group table (sanitised first rows, running tile counts) is built
+// in shared memory by build_group_table.
+// ---------------------------------------------------------------------------------------------
+struct GroupTable {
+    const uint32_t* first; // groups + 1 row offsets
+    const uint32_t* tiles; // groups + 1 running counts of ragged tiles (ragged rows only)
+};
+
+// By one warp.
+__device__ __forceinline__ void build_group_table(const EpilogueParams& ep, uint32_t tile, uint32_t* first, uint32_t* tiles)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t       top = 0u, before = 0u;
+    for (uint32_t g0 = 0; g0 <= ep.groups; g0 += 32u) {
+        const uint32_t g = g0 + lane;
+        const uint32_t v = g <= ep.groups ? clamp_offset(__ldg(ep.offsets + g), ep.rows) : 0u;
+        const uint32_t m = max(warp_scan_max(v, lane), top); // first row of group g
+        uint32_t       prev = __shfl_up_sync(0xffffffffu, m, 1);
+        if (lane == 0) prev = g0 ? top : m;
+        const uint32_t n    = (m - prev + tile - 1u) / tile; // tiles of group g - 1
+        const uint32_t incl = before + warp_scan_add(n, lane);
+        if (g <= ep.groups) {
+            first[g] = m;
+            tiles[g] = incl;
+        }
+        top    = __shfl_sync(0xffffffffu, m, 31);
+        before = __shfl_sync(0xffffffffu, incl, 31);
+    }
+}
+
+template <bool TR>
+__device__ __forceinline__ bool work_next_epilogue(const GemmParams& p, const EpilogueParams& ep, const GroupTable& gt,
+                                                   WorkCursor& cur, uint32_t unit, uint32_t units, int bn, int bm,
+                                                   WorkCoord& c)
+{
+    if (ep.ragged == RAGGED_NONE) {
+        if (!work_next(p, cur, unit, units, bn, bm, c)) return false;
+        c.z_a = c.z_b = c.z_in;
+        c.k_first = c.group = c.first = 0u;
+        c.end     = TR ? p.N : p.M;
+        return true;
+    }
+    if (ep.ragged == RAGGED_K) {
+        if (!work_next(p, cur, unit, units, bn, bm, c)) return false;
+        c.group = c.z_in; // (the batch index)
+        c.first = c.k_first = gt.first[c.group];
+        c.z_a = c.z_b = 0u;
+        c.end = p.M;
+        c.kb0 = 0u;
+        c.kb1 = (gt.first[c.group + 1u] - c.first + BLOCK_K - 1u) / BLOCK_K;
+        return true;
+    }
+    const uint32_t other = TR ? p.m_tiles : p.n_tiles; // tiles of the other extent
+    const uint32_t w     = cur.next;
+    if (w >= gt.tiles[ep.groups] * other) return false;
+    cur.next += units;
+    uint32_t       lo = 0u, hi = ep.groups; // the group whose tiles [tiles[e], tiles[e + 1]) x other hold w
+    const uint32_t wt = w / other;
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) / 2u;
+        if (gt.tiles[mid] <= wt) lo = mid;
+        else hi = mid;
+    }
+    const uint32_t in_g  = w - gt.tiles[lo] * other;
+    const uint32_t rt    = gt.tiles[lo + 1u] - gt.tiles[lo];
+    const uint32_t o     = in_g / rt;
+    c.group              = lo;
+    c.first              = gt.first[lo];
+    c.end                = gt.first[lo + 1u];
+    const uint32_t along = c.first + (in_g - o * rt) * static_cast<uint32_t>(TR ? bn : bm);
+    c.m0                 = TR ? o * static_cast<uint32_t>(bm) : along;
+    c.n0                 = TR ? along : o * static_cast<uint32_t>(bn);
+    c.z_a                = TR ? lo : 0u;
+    c.z_b                = TR ? 0u : lo;
+    c.z_in = c.z_out = 0u;
+    c.k_first = c.partial = 0u;
+    c.kb0                 = 0u;
+    c.kb1                 = p.k_blocks;
+    return true;
+}
+
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
                                              uint32_t d)
 {
@@ -467,10 +563,379 @@ __device__ __forceinline__ uint32_t pack2(uint32_t lo_bits, uint32_t hi_bits)
 //
 // Edges: TMA zero-fills out-of-range loads (M, N and K tails) and clips stores.
 // No TMA load here uses cluster multicast.
+//
+// EP: a product with an epilogue, dense or grouped (epilogue.cuh has the mathematics).  Eight
+// epilogue warps, two per lane quarter, take the column chunks of a tile alternately: an
+// activation costs 15 to 40 instructions per element, and four warps alone would pace short K
+// loops.  The matrix an epilogue reads (residual, or Z in gradient mode) comes by TMA into the
+// staging buffer its chunk will leave from, requested before the accumulator is awaited, so its
+// latency hides under the main loop; Z leaves through a staging buffer of its own.
 // ---------------------------------------------------------------------------------------------
-template <int BN, int OUT, int CL, bool TR, bool GATHER, bool KS = false>
+// Maps of the matrices beside C: the one the epilogue reads, and where Z goes.
+struct EpilogueMaps {
+    CUtensorMap in, aux;
+};
+
+// Sum of v[j] over the 32 lanes, for 32 values of j: lane j receives the sum of v[j].
+__device__ __forceinline__ float warp_column_sums(float (&v)[32], uint32_t lane)
+{
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) {
+        const bool up = (lane & s) != 0u;
+#pragma unroll
+        for (int i = 0; i < s; ++i) {
+            const float send = up ? v[i] : v[i + s];
+            const float keep = up ? v[i + s] : v[i];
+            v[i]             = keep + __shfl_xor_sync(0xffffffffu, send, s);
+        }
+    }
+    return v[0];
+}
+
+template <int OUT>
+using OutType = std::conditional_t<OUT == OUT_F32, float, std::conditional_t<OUT == OUT_F16, __half, __nv_bfloat16>>;
+
+// 16 bytes of an output type as f32 values and back.
+template <int OUT>
+__device__ __forceinline__ void unpack16(const uint32_t (&w)[4], float* v)
+{
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (OUT == OUT_F32) {
+            v[k] = __uint_as_float(w[k]);
+        } else if constexpr (OUT == OUT_F16) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+            v[2 * k] = f.x, v[2 * k + 1] = f.y;
+        } else {
+            v[2 * k] = __uint_as_float(w[k] << 16), v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        }
+    }
+}
+
+template <int OUT>
+__device__ __forceinline__ void pack16(const float* v, uint32_t (&w)[4])
+{
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (OUT == OUT_F32) w[k] = __float_as_uint(v[k]);
+        else w[k] = pack2<OUT>(__float_as_uint(v[2 * k]), __float_as_uint(v[2 * k + 1]));
+    }
+}
+
+// One epilogue warp of a staged kernel with an epilogue: 32 rows x 128-byte column chunks.
+template <int OUT>
+struct EpilogueWarp {
+    using T = OutType<OUT>;
+    static constexpr int      CH    = OUT == OUT_F32 ? 32 : 64; // columns per chunk
+    static constexpr int      PARTS = CH / 32;
+    static constexpr uint32_t UNIT  = CH / 8;                   // columns per 16 bytes
+
+    const GemmParams&        p;
+    const EpilogueParams&    ep;
+    const EpilogueMaps&      em;
+    const CUtensorMap&       tmD;
+    void*                    out;     // C, for rows that may not be stored 32 at a time
+    uint32_t                 lane;
+    uint32_t                 stg;     // staging buffers: ep.bufs for C, then one for Z
+    uint32_t                 in_bar;  // barriers of the first two
+    uint8_t*                 bias_sm; // CH biases in C's type (128 bytes)
+    volatile uint32_t*       s_abort;
+    uint32_t                 count     = 0; // chunks so far: the next one's buffer is count % ep.bufs
+    uint32_t                 in_phase  = 0; // parity per buffer
+    uint32_t                 in_flight = 0; // requested, not yet awaited
+    T                        bias_reg[PARTS]; // this lane's biases of the next chunk
+
+    __device__ __forceinline__ uint32_t slot(uint32_t k) const { return (count + k) & (ep.bufs - 1u); }
+
+    // Requests the read matrix's chunk k chunks ahead.  Its buffer must have been read by the
+    // stores before (request() is called after a wait on them).
+    __device__ __forceinline__ void request(uint32_t k, uint32_t row0, uint32_t col0, uint32_t z)
+    {
+        const uint32_t b = slot(k);
+        if (lane == 0) {
+            ptx::mbar_expect_tx(in_bar + 8u * b, EPI_BUF_BYTES);
+            ptx::tma_load_3d(stg + b * EPI_BUF_BYTES, &em.in, in_bar + 8u * b, col0, row0, z, 0);
+        }
+        in_flight |= 1u << b;
+    }
+
+    // Every store so far has read its staging buffer, and this warp's own accesses to them are done.
+    __device__ __forceinline__ void buffers_free()
+    {
+        ptx::fence_proxy_async_smem();
+        if (lane == 0) ptx::tma_store_wait_read<0>();
+        __syncwarp();
+    }
+
+    __device__ __forceinline__ void prefetch_bias(const WorkCoord& c, uint32_t col0)
+    {
+        if (!ep.bias || ep.bias_on_rows) return;
+        const T* b = static_cast<const T*>(ep.bias) + (ep.ragged == RAGGED_ROWS ? c.group : c.z_in) * ep.bias_stride;
+#pragma unroll
+        for (int h = 0; h < PARTS; ++h) {
+            const uint32_t col = col0 + h * 32u + lane;
+            bias_reg[h]        = col < p.N ? __ldg(b + col) : from_f32<T>(0.f);
+        }
+    }
+
+    __device__ __forceinline__ float row_bias(const WorkCoord& c, uint32_t row) const
+    {
+        if (!ep.bias || !ep.bias_on_rows || row >= p.M) return 0.f;
+        return to_f32(__ldg(static_cast<const T*>(ep.bias) + c.z_in * ep.bias_stride + row));
+    }
+
+    __device__ __forceinline__ void store_row_from(uint32_t rowaddr, void* base, uint32_t row, uint32_t col0) const
+    {
+#pragma unroll
+        for (uint32_t u = 0; u < 8; ++u) {
+            if (col0 + u * UNIT < p.N) {
+                uint4 w;
+                ptx::ld_shared_v4(rowaddr + ((u ^ (lane & 7u)) << 4), w.x, w.y, w.z, w.w);
+                *reinterpret_cast<uint4*>(static_cast<T*>(base) + static_cast<uint64_t>(row) * p.N + col0 + u * UNIT) = w;
+            }
+        }
+    }
+
+    // The chunk at (row0, col0) from its accumulators; `end` bounds the rows.  False: a wait ran out.
+    __device__ __forceinline__ bool finish(const WorkCoord& c, uint32_t row0, uint32_t col0, uint32_t end, float bias_row,
+                                           const uint32_t (&a)[CH])
+    {
+        const uint32_t b    = slot(0);
+        const uint32_t sbuf = stg + b * EPI_BUF_BYTES, rowaddr = sbuf + lane * 128u;
+        const uint32_t xbuf = stg + ep.bufs * EPI_BUF_BYTES, xrow = xbuf + lane * 128u;
+        const uint32_t row  = row0 + lane;
+        const bool     col_bias = ep.bias && !ep.bias_on_rows;
+        if (col_bias) {
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) reinterpret_cast<T*>(bias_sm)[h * 32 + lane] = bias_reg[h];
+        }
+        if (ep.streamed) {
+            bool ok = bounded_wait(in_bar + 8u * b, (in_phase >> b) & 1u, s_abort, p.status, ST_EPI_WAIT);
+            ok      = __all_sync(0xffffffffu, ok);
+            if (!ok) return false;
+            in_phase ^= 1u << b;
+            in_flight &= ~(1u << b);
+        }
+        // the buffers written below must have been read by the stores that last used them
+        if (lane == 0) {
+            if (ep.aux || ep.bufs == 1u) ptx::tma_store_wait_read<0>();
+            else if (!ep.streamed) ptx::tma_store_wait_read<1>();
+        }
+        __syncwarp();
+        float row_sum = 0.f;
+#pragma unroll
+        for (int h = 0; h < PARTS; ++h) {
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(a[h * 32 + j]);
+            // 16-byte unit i of this half's columns within the row's 128 bytes (128-byte swizzle)
+            constexpr uint32_t UNITS = 32 / UNIT;
+            auto at = [&](uint32_t i) { return ((h * UNITS + i) ^ (lane & 7u)) << 4; };
+            if (ep.gradient) {
+                if (ep.streamed) {
+                    with_act(ep.act, [&](auto tag) {
+                        constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll
+                        for (uint32_t i = 0; i < UNITS; ++i) {
+                            uint32_t w[4];
+                            float    z[UNIT];
+                            ptx::ld_shared_v4(rowaddr + at(i), w[0], w[1], w[2], w[3]);
+                            unpack16<OUT>(w, z);
+#pragma unroll
+                            for (uint32_t j = 0; j < UNIT; ++j)
+                                v[i * UNIT + j] = __fmul_rn(v[i * UNIT + j], act_slope<ACT>(z[j], ep.c0, ep.c1));
+                        }
+                    });
+                }
+            } else {
+                if (col_bias) {
+#pragma unroll
+                    for (uint32_t i = 0; i < UNITS; ++i) {
+                        uint32_t w[4];
+                        float    t[UNIT];
+                        ptx::ld_shared_v4(ptx::smem_u32(bias_sm) + (h * UNITS + i) * 16u, w[0], w[1], w[2], w[3]);
+                        unpack16<OUT>(w, t);
+#pragma unroll
+                        for (uint32_t j = 0; j < UNIT; ++j) v[i * UNIT + j] += t[j];
+                    }
+                } else if (ep.bias) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] += bias_row;
+                }
+                if (ep.aux) {
+#pragma unroll
+                    for (uint32_t i = 0; i < UNITS; ++i) {
+                        uint32_t w[4];
+                        pack16<OUT>(v + i * UNIT, w);
+                        st_shared_v4(xrow + at(i), w[0], w[1], w[2], w[3]);
+                    }
+                }
+                with_act(ep.act, [&](auto tag) {
+                    constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = act_value<ACT>(v[j], ep.c0, ep.c1);
+                });
+                if (ep.streamed) {
+#pragma unroll
+                    for (uint32_t i = 0; i < UNITS; ++i) {
+                        uint32_t w[4];
+                        float    r[UNIT];
+                        ptx::ld_shared_v4(rowaddr + at(i), w[0], w[1], w[2], w[3]);
+                        unpack16<OUT>(w, r);
+#pragma unroll
+                        for (uint32_t j = 0; j < UNIT; ++j) v[i * UNIT + j] += r[j];
+                    }
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < UNITS; ++i) {
+                uint32_t w[4];
+                pack16<OUT>(v + i * UNIT, w);
+                st_shared_v4(rowaddr + at(i), w[0], w[1], w[2], w[3]);
+            }
+            if (ep.part) {
+                // (what lies outside C may be NaN: a zero-filled operand times an infinity)
+                if (ep.bias_on_rows) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) row_sum += col0 + h * 32 + j < p.N ? v[j] : 0.f;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = row < end ? v[j] : 0.f;
+                    const float    sum   = warp_column_sums(v, lane);
+                    const uint32_t block = ep.ragged == RAGGED_ROWS
+                                               ? group_first_block(c.first, c.group, 32u) + (row0 - c.first) / 32u
+                                               : c.z_out * ep.part_blocks + row0 / 32u;
+                    const uint32_t col   = col0 + h * 32u + lane;
+                    if (col < p.N) ep.part[static_cast<uint64_t>(block) * p.N + col] = sum;
+                }
+            }
+        }
+        if (ep.part && ep.bias_on_rows && row < end)
+            ep.part[(static_cast<uint64_t>(c.z_out) * ep.part_blocks + col0 / CH) * p.M + row] = row_sum;
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (ep.ragged == RAGGED_ROWS && row0 + 32u > end) {
+            // the block's last rows belong to the next group: row by row, straight from the buffer
+            if (row < end) {
+                store_row_from(rowaddr, out, row, col0);
+                if (ep.aux) store_row_from(xrow, ep.preact, row, col0);
+            }
+        } else if (lane == 0) {
+            ptx::tma_store_3d(&tmD, sbuf, col0, row0, c.z_out, 0);
+            if (ep.aux) ptx::tma_store_3d(&em.aux, xbuf, col0, row0, c.z_out, 0);
+        }
+        if (lane == 0) ptx::tma_store_commit(); // (an empty group keeps the count of the waits above)
+        ++count;
+        return true;
+    }
+
+    // After a give-up: the loads still in flight must land before this CTA's memory goes away.
+    __device__ __forceinline__ void drain()
+    {
+        if (lane == 0) {
+            for (uint32_t b = 0; b < 2u; ++b) {
+                if (!((in_flight >> b) & 1u)) continue;
+                const uint64_t t0 = ptx::global_timer_ns();
+                while (!ptx::mbar_try_wait(in_bar + 8u * b, (in_phase >> b) & 1u)) {
+                    if (ptx::global_timer_ns() - t0 > WAIT_LIMIT_NS) {
+                        atomicOr(p.status, ST_DRAIN_WAIT);
+                        break;
+                    }
+                }
+            }
+            ptx::tma_store_wait_read<0>();
+        }
+    }
+};
+
+// The transposing epilogue's part of a tile with an epilogue: `n` <= 32 columns from col0 on of
+// kernel row i (this lane's), D(i, j) lying at out[j * M + i].  `side`: the read matrix's values.
+template <int OUT>
+struct EpilogueColumns {
+    using T = OutType<OUT>;
+    const GemmParams&     p;
+    const EpilogueParams& ep;
+    uint32_t              lane;
+
+    __device__ __forceinline__ uint64_t at(const WorkCoord& c, uint32_t col, uint32_t i) const
+    {
+        return (static_cast<uint64_t>(c.z_out) * p.N + col) * p.M + i;
+    }
+
+    __device__ __forceinline__ void load_side(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, float (&side)[32]) const
+    {
+        const T* src = static_cast<const T*>(ep.gradient ? ep.preact : ep.residual);
+#pragma unroll
+        for (uint32_t r = 0; r < 32; ++r) side[r] = live && r < n ? to_f32(src[at(c, col0 + r, i)]) : 0.f;
+    }
+
+    // `block`: where a sum along the columns goes; `block_rows`: where sums over the rows go.
+    __device__ __forceinline__ void finish(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, uint32_t block,
+                                           uint32_t block_rows, const uint32_t (&a)[32], const float (&side)[32]) const
+    {
+        float v[32];
+#pragma unroll
+        for (int r = 0; r < 32; ++r) v[r] = __uint_as_float(a[r]);
+        if (ep.gradient) {
+            if (ep.streamed)
+                with_act(ep.act, [&](auto tag) {
+                    constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll
+                    for (int r = 0; r < 32; ++r) v[r] = __fmul_rn(v[r], act_slope<ACT>(side[r], ep.c0, ep.c1));
+                });
+        } else {
+            if (ep.bias) {
+                const T* bias = static_cast<const T*>(ep.bias) + (ep.ragged == RAGGED_ROWS ? c.group : c.z_in) * ep.bias_stride;
+                if (ep.bias_on_rows) {
+                    const float b = live ? to_f32(__ldg(bias + i)) : 0.f;
+#pragma unroll
+                    for (int r = 0; r < 32; ++r) v[r] += b;
+                } else {
+#pragma unroll
+                    for (uint32_t r = 0; r < 32; ++r) v[r] += r < n ? to_f32(__ldg(bias + col0 + r)) : 0.f;
+                }
+            }
+            if (ep.aux && live) {
+                T* pre = static_cast<T*>(ep.preact);
+#pragma unroll
+                for (uint32_t r = 0; r < 32; ++r)
+                    if (r < n) pre[at(c, col0 + r, i)] = from_f32<T>(v[r]);
+            }
+            with_act(ep.act, [&](auto tag) {
+                constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll
+                for (int r = 0; r < 32; ++r) v[r] = act_value<ACT>(v[r], ep.c0, ep.c1);
+            });
+            if (ep.streamed) {
+#pragma unroll
+                for (int r = 0; r < 32; ++r) v[r] += side[r];
+            }
+        }
+        if (live) {
+            T* out = static_cast<T*>(p.out);
+#pragma unroll
+            for (uint32_t r = 0; r < 32; ++r)
+                if (r < n) out[at(c, col0 + r, i)] = from_f32<T>(v[r]);
+        }
+        if (!ep.part) return;
+        if (ep.bias_on_rows) {
+            float sum = 0.f;
+#pragma unroll
+            for (uint32_t r = 0; r < 32; ++r) sum += r < n ? v[r] : 0.f;
+            if (live) ep.part[static_cast<uint64_t>(block) * p.M + i] = sum;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 32; ++r) v[r] = live ? v[r] : 0.f;
+            const float sum = warp_column_sums(v, lane);
+            if (lane < n) ep.part[static_cast<uint64_t>(block_rows) * p.N + col0 + lane] = sum;
+        }
+    }
+};
+
+template <int BN, int OUT, int CL, bool TR, bool GATHER, bool KS = false, bool EP = false>
 __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUtensorMap& tmB,
-                                               const CUtensorMap* tmDs, const CUtensorMap& tmW, const GemmParams& p)
+                                               const CUtensorMap* tmDs, const CUtensorMap& tmW, const GemmParams& p,
+                                               const EpilogueMaps* em = nullptr, const EpilogueParams* epp = nullptr)
 {
     const CUtensorMap& tmD = tmDs[0];
     static_assert(BN == 16 || BN == 32 || BN == 64 || BN == 128 || BN == 256 || BN == 512,
@@ -517,6 +982,10 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
     __shared__ __align__(8) uint64_t s_drain;
     __shared__ uint32_t              s_tmem_base;
     __shared__ volatile uint32_t     s_abort;
+    static_assert(!EP || !GATHER, "no gathering kernels with an epilogue");
+    constexpr int                    EPW = EP ? EPI_WARPS : 4; // epilogue warps
+    __shared__ __align__(8) uint64_t s_in[EP && !TR ? EPI_WARPS * 2 : 1];                // EP: chunk of the read matrix landed
+    __shared__ __align__(16) uint8_t s_bias[EP && !TR ? EPI_WARPS * 128 : 16];           // EP: a chunk's biases, per warp
 
     const uint32_t tid    = threadIdx.x;
     const uint32_t warp   = tid >> 5;
@@ -553,6 +1022,22 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
 
     const uint32_t ring = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u; // ring of operand tiles
     const uint32_t epi  = ring + stages * pitch;                      // epilogue staging (unused when TR)
+    GroupTable     gt{nullptr, nullptr};
+    if constexpr (EP) { // the group table lies at the very end of the dynamic shared memory
+        if (epp->ragged != RAGGED_NONE) {
+            uint32_t* tab = reinterpret_cast<uint32_t*>(smem_raw + epp->table_at);
+            gt.first      = tab;
+            gt.tiles      = tab + epp->groups + 1u;
+            if (warp == 2) {
+                ptx::grid_dep_wait(); // the offsets may come from the kernel before this one
+                build_group_table(*epp, TR ? static_cast<uint32_t>(BN) : tile_m, tab, tab + epp->groups + 1u);
+            }
+        }
+    }
+    auto next_work = [&](WorkCursor& cur, WorkCoord& c) -> bool {
+        if constexpr (EP) return work_next_epilogue<TR>(p, *epp, gt, cur, unit, units, wn, tile_m, c);
+        else return work_next(p, cur, unit, units, wn, tile_m, c);
+    };
 
     if (warp == 0) {
         // Barrier set-up spread over the lanes of warp 0 (one thread doing all of it serially is
@@ -574,7 +1059,10 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
         }
         if (lane >= 30u) {
             ptx::mbar_init(ptx::smem_u32(&s_tfull[lane - 30u]), 1);
-            ptx::mbar_init(ptx::smem_u32(&s_tempty[lane - 30u]), 4 * CL);
+            ptx::mbar_init(ptx::smem_u32(&s_tempty[lane - 30u]), EPW * CL);
+        }
+        if constexpr (EP && !TR) {
+            if (lane < EPI_WARPS * 2) ptx::mbar_init(ptx::smem_u32(&s_in[lane]), 1);
         }
         ptx::fence_mbar_init();
     }
@@ -620,7 +1108,21 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             const uint64_t pol_b = ptx::make_l2_policy((p.l2_hints >> 2) & 3u);
             WorkCursor cur = work_begin(p, unit, krank);
             WorkCoord  c;
-            for (uint32_t w = unit; ok && work_next(p, cur, unit, units, wn, tile_m, c); w += units) {
+            const CUtensorMap* mapA = &tmA;
+            const CUtensorMap* mapB = &tmB;
+            for (uint32_t w = unit; ok && next_work(cur, c); w += units) {
+                if constexpr (EP) {
+                    if (epp->ragged == RAGGED_K) { // this group's own maps, written by the kernel before this one
+                        mapA = epp->maps + 2u * c.group;
+                        mapB = mapA + 1;
+                        dep_wait();
+                        ptx::fence_tensormap_acquire(mapA);
+                        ptx::fence_tensormap_acquire(mapB);
+                    }
+                } else {
+                    c.z_a = c.z_b = c.z_in;
+                    c.k_first = 0u;
+                }
                 const int32_t   am = static_cast<int32_t>(c.m0 + rank * BLOCK_M);
                 const int32_t   bn = static_cast<int32_t>(c.n0 + rank * sub_rows);
                 // Streaming (HBM-bound) problems rotate each work unit's K order so that the CTAs
@@ -645,7 +1147,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         const uint32_t rel = i + rot >= nst ? i + rot - nst : i + rot;
                         const int32_t  kb  = ileave ? static_cast<int32_t>((krank + rel * 2u) * kc)
                                                     : static_cast<int32_t>(c.kb0 + rel * kc);
-                        const int32_t  k0  = kb * BLOCK_K;
+                        const int32_t  k0  = kb * BLOCK_K + static_cast<int32_t>(c.k_first);
                         ok = bounded_wait(ptx::smem_u32(&s_empty[stage]), phase ^ 1u, &s_abort,
                                           p.status, ST_PRODUCER_WAIT);
                         if (!ok) break;
@@ -660,19 +1162,19 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                             B200_TL_CTA(0);
                         }
                         if (p.a_mn_major == 0u) {
-                            if (p.k4d) ptx::tma_load_4d(sa, &tmA, bar, 0, am, kb, c.z_in, pol_a);
-                            else ptx::tma_load_3d(sa, &tmA, bar, k0, am, c.z_in, pol_a);
+                            if (p.k4d) ptx::tma_load_4d(sa, mapA, bar, 0, am, kb, c.z_a, pol_a);
+                            else ptx::tma_load_3d(sa, mapA, bar, k0, am, c.z_a, pol_a);
                         } else {
-                            ptx::tma_load_3d(sa, &tmA, bar, am, k0, c.z_in, pol_a);
-                            if (p.bm > 64u) ptx::tma_load_3d(sa + half, &tmA, bar, am + 64, k0, c.z_in, pol_a);
+                            ptx::tma_load_3d(sa, mapA, bar, am, k0, c.z_a, pol_a);
+                            if (p.bm > 64u) ptx::tma_load_3d(sa + half, mapA, bar, am + 64, k0, c.z_a, pol_a);
                         }
                         if (p.b_mn_major == 0u) {
-                            if (p.k4d) ptx::tma_load_4d(sb, &tmB, bar, 0, bn, kb, c.z_in, pol_b);
-                            else ptx::tma_load_3d(sb, &tmB, bar, k0, bn, c.z_in, pol_b);
+                            if (p.k4d) ptx::tma_load_4d(sb, mapB, bar, 0, bn, kb, c.z_b, pol_b);
+                            else ptx::tma_load_3d(sb, mapB, bar, k0, bn, c.z_b, pol_b);
                         } else {
 #pragma unroll
                             for (int j = 0; j < SUB_ROWS / 64; ++j)
-                                ptx::tma_load_3d(sb + j * half, &tmB, bar, bn + j * 64, k0, c.z_in, pol_b);
+                                ptx::tma_load_3d(sb + j * half, mapB, bar, bn + j * 64, k0, c.z_b, pol_b);
                         }
                         if (issued == 0) B200_TL(4);
                         ++issued;
@@ -697,7 +1199,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                     if (!ok) break;
                     const uint32_t sa = ring + stage * pitch;
                     const uint32_t sb = sa + a_bytes;
-                    const int32_t  k0 = static_cast<int32_t>(kb * BLOCK_K);
+                    const int32_t  k0 = static_cast<int32_t>(kb * BLOCK_K + c.k_first);
                     const uint32_t step_bytes = a_bytes + nsub * sub_bytes; // this CTA's share
                     uint32_t       bar = ptx::smem_u32(&s_full[stage]);
                     if constexpr (CL == 2) {
@@ -714,12 +1216,12 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         B200_TL_CTA(0);
                     }
                     if (p.a_mn_major == 0u) {
-                        tma_load<CL>(sa, &tmA, bar, k0, am, c.z_in, pol_a);
+                        tma_load<CL>(sa, mapA, bar, k0, am, c.z_a, pol_a);
                     } else {
 #pragma unroll
                         for (int j = 0; j < BLOCK_M / 64; ++j)
-                            tma_load<CL>(sa + j * (64 * BLOCK_K * 2), &tmA, bar, am + j * 64, k0,
-                                         c.z_in, pol_a);
+                            tma_load<CL>(sa + j * (64 * BLOCK_K * 2), mapA, bar, am + j * 64, k0,
+                                         c.z_a, pol_a);
                     }
 #pragma unroll
                     for (int h = 0; h < NSUB; ++h) {
@@ -727,13 +1229,13 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         const int32_t  bh = bn + h * UMMA_N; // first B' row of sub-tile h
                         const uint32_t sh = sb + h * SUB_BYTES;
                         if (p.b_mn_major == 0u) {
-                            tma_load<CL>(sh, &tmB, bar, k0, bh, c.z_in, pol_b);
+                            tma_load<CL>(sh, mapB, bar, k0, bh, c.z_b, pol_b);
                         } else {
 #pragma unroll
                             for (int j = 0; j < SUB_ROWS / 64; ++j)
                                 if (!FLEX || static_cast<uint32_t>(j) * 64u < sub_rows)
-                                    tma_load<CL>(sh + j * (64 * BLOCK_K * 2), &tmB, bar, bh + j * 64,
-                                                 k0, c.z_in, pol_b);
+                                    tma_load<CL>(sh + j * (64 * BLOCK_K * 2), mapB, bar, bh + j * 64,
+                                                 k0, c.z_b, pol_b);
                         }
                     }
                     if (issued == 0) B200_TL(4);
@@ -777,7 +1279,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             bool           ok = true;
             WorkCursor cur = work_begin(p, unit, krank);
             WorkCoord  c;
-            for (; ok && work_next(p, cur, unit, units, wn, tile_m, c); ++it) {
+            for (; ok && next_work(cur, c); ++it) {
                 if constexpr (NSUB == 2) {
                     // Two column halves with their own full / empty barriers (s_tfull[h],
                     // s_tempty[h]), staggered by stg_x k-blocks: see TileStep.  Three
@@ -913,6 +1415,136 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                 }
             }
             B200_TL(8);
+        }
+    } else if constexpr (EP) {
+        // ------------------------------------------------------------------ epilogue with activation, bias, ...
+        const uint32_t q  = warp & 3u;          // TMEM lane quarter this warp may read
+        const uint32_t hw = (warp - 2u) >> 2;   // takes column chunks hw, hw + 2, ...
+        uint32_t       it = 0;
+        bool           ok = true;
+        WorkCursor     cur = work_begin(p, unit, krank);
+        WorkCoord      c;
+        auto release = [&](uint32_t bar_i) { // this warp has read its part of the accumulator
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CL == 2) ptx::mbar_arrive_cluster(ptx::smem_u32(&s_tempty[bar_i]), 0);
+                else ptx::mbar_arrive(ptx::smem_u32(&s_tempty[bar_i]));
+            }
+        };
+        auto accumulator = [&](uint32_t bar_i, uint32_t parity) -> bool {
+            bool r = bounded_wait(ptx::smem_u32(&s_tfull[bar_i]), parity, &s_abort, p.status, ST_EPI_WAIT);
+            r      = __all_sync(0xffffffffu, r);
+            ptx::tc_fence_after();
+            return r;
+        };
+        if constexpr (KS) {
+            // one tile per cluster; the partials are summed after the cluster barriers below
+            if (next_work(cur, c)) {
+                ok    = accumulator(0u, 0u);
+                ks_c  = c;
+                ks_ok = ok;
+            }
+        } else if constexpr (TR) {
+            const EpilogueColumns<OUT> ec{p, *epp, lane};
+            constexpr uint32_t         CHUNKS = (BN + 31) / 32;
+            const uint32_t             bs     = BN < 32 ? BN : 32; // columns per block of sums
+            for (; ok && next_work(cur, c); ++it) {
+                const uint32_t buf  = it % NUM_ACC;
+                const uint32_t i    = c.m0 + q * 32u + lane;
+                const bool     live = (q * 32u + lane) < p.bm && i < p.M;
+                const uint32_t tacc = tmem_base + ((q * 32u) << 16) + buf * ACC_COLS;
+                bool           seen = false;
+                dep_wait();
+#pragma unroll 1
+                for (uint32_t ch = hw; ch < CHUNKS; ch += 2u) {
+                    const uint32_t col0 = c.n0 + ch * 32u;
+                    const uint32_t n    = col0 < c.end ? min(min(32u, BN - ch * 32u), c.end - col0) : 0u;
+                    float          side[32];
+                    if (epp->streamed) ec.load_side(c, col0, n, i, live, side);
+                    if (!seen) {
+                        ok = accumulator(buf, (it / NUM_ACC) & 1u);
+                        if (!ok) break;
+                        seen = true;
+                    }
+                    uint32_t v[32];
+                    ptx::tmem_ld_32x32(tacc + ch * 32u, v);
+                    ptx::tmem_ld_wait(v);
+                    if (ch + 2u >= CHUNKS) release(buf);
+                    if (n == 0u) continue;
+                    const uint32_t block = epp->ragged == RAGGED_ROWS
+                                               ? group_first_block(c.first, c.group, bs) + (col0 - c.first) / bs
+                                               : c.z_out * epp->part_blocks + col0 / bs;
+                    ec.finish(c, col0, n, i, live, block, c.z_out * epp->part_blocks + c.m0 / p.bm * 4u + q, v, side);
+                }
+                if (ok && !seen) { // fewer chunks than warps
+                    ok = accumulator(buf, (it / NUM_ACC) & 1u);
+                    if (ok) release(buf);
+                }
+            }
+        } else {
+            using EW = EpilogueWarp<OUT>;
+            const uint32_t per_warp = (epp->bufs + epp->aux) * EPI_BUF_BYTES;
+            EW ew{p, *epp, *em, tmD, p.out, lane, epi + (warp - 2u) * per_warp, ptx::smem_u32(&s_in[(warp - 2u) * 2u]),
+                  &s_bias[(warp - 2u) * 128u], &s_abort};
+            for (; ok && next_work(cur, c); ++it) {
+                const uint32_t buf = it % NUM_ACC;
+#pragma unroll 1
+                for (uint32_t hh = 0; hh < static_cast<uint32_t>(NSUB); ++hh) {
+                    const uint32_t bar_i  = (NSUB == 2) ? hh : buf;
+                    const uint32_t parity = (NSUB == 2) ? (it & 1u) : ((it / NUM_ACC) & 1u);
+                    const uint32_t colh   = c.n0 + hh * UMMA_N;
+                    const uint32_t row0   = c.m0 + rank * BLOCK_M + q * 32u;
+                    const uint32_t width  = FLEX ? wn : static_cast<uint32_t>(UMMA_N);
+                    const uint32_t live   = (row0 < c.end && q * 32u < p.bm && colh < p.N) ? (min(width, p.N - colh) + EW::CH - 1u) / EW::CH : 0u;
+                    const uint32_t mine   = live > hw ? (live - hw + 1u) / 2u : 0u; // this warp's chunks: hw, hw + 2, ...
+                    auto           col    = [&](uint32_t k) { return colh + (hw + 2u * k) * EW::CH; };
+                    const uint32_t tacc   = tmem_base + ((q * 32u) << 16) + (NSUB == 2 ? hh * UMMA_N : buf * ACC_COLS);
+                    float          bias_row = 0.f;
+                    if (mine) {
+                        dep_wait();
+                        if (epp->streamed) {
+                            ew.buffers_free();
+                            for (uint32_t k = 0; k < min(epp->bufs, mine); ++k) ew.request(k, row0, col(k), c.z_out);
+                        }
+                        ew.prefetch_bias(c, col(0));
+                        bias_row = ew.row_bias(c, row0 + lane);
+                    }
+                    ok = accumulator(bar_i, parity);
+                    if (!ok) break;
+                    if (mine == 0u) release(bar_i);
+#pragma unroll 1
+                    for (uint32_t k = 0; k < mine; ++k) {
+                        uint32_t a[EW::CH];
+                        if (c.kb1 > c.kb0) {
+                            uint32_t (&a0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&a[0]);
+                            ptx::tmem_ld_32x32(tacc + (hw + 2u * k) * EW::CH, a0);
+                            if constexpr (EW::CH == 64) {
+                                uint32_t (&a1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&a[32]);
+                                ptx::tmem_ld_32x32(tacc + (hw + 2u * k) * EW::CH + 32u, a1);
+                                ptx::tmem_ld_wait(a0);
+                                ptx::tmem_ld_wait(a1);
+                            } else {
+                                ptx::tmem_ld_wait(a0);
+                            }
+                        } else { // no rows to sum over
+#pragma unroll
+                            for (int j = 0; j < EW::CH; ++j) a[j] = 0u;
+                        }
+                        if (k + 1u == mine) release(bar_i);
+                        if (epp->streamed && k > 0u && k - 1u + epp->bufs < mine) {
+                            ew.buffers_free(); // the chunk before this one left from the buffer asked for now
+                            ew.request(epp->bufs - 1u, row0, col(k - 1u + epp->bufs), c.z_out);
+                        }
+                        __syncwarp(); // (the biases of the chunk before have been read)
+                        ok = ew.finish(c, row0, col(k), c.end, bias_row, a);
+                        if (!ok) break;
+                        if (k + 1u < mine) ew.prefetch_bias(c, col(k + 1u));
+                    }
+                    if (!ok) break;
+                }
+            }
+            ew.drain();
         }
     } else {
         // ------------------------------------------------------------------ epilogue
@@ -1111,6 +1743,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
         const uint32_t ks   = p.split_k;
         const uint32_t q    = warp & 3u;
         const uint32_t tacc = tmem_base + ((q * 32u) << 16);
+        const uint32_t hw   = EP && warp >= 2u ? (warp - 2u) >> 2 : 0u; // EP: two warps per quarter, a rank's chunks dealt alternately
         __syncwarp();
         if (warp == 2 && lane == 0) B200_TL(16);
         ptx::cluster_arrive();
@@ -1121,6 +1754,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             for (uint32_t ch = 0; ch < static_cast<uint32_t>(NCH); ++ch) {
                 const uint32_t owner = ch % ks;
                 if (owner == krank) continue;
+                if (EP && ((ch / ks) & 1u) != hw) continue;
                 // (within a warp's slot the 16-byte units are laid out [unit][lane]: every store and
                 // load instruction of the warp covers 512 contiguous bytes)
                 const uint32_t local  = ring + (((ch / ks) * ks + krank) * 4u + q) * WSLOT + lane * 16u;
@@ -1146,8 +1780,16 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             const uint32_t row0     = ks_c.m0 + q * 32u;
             const bool     row_live = row0 < p.M;
             uint32_t       nstore   = 0;
+            [[maybe_unused]] const uint32_t per_warp = EP ? (epp->bufs + epp->aux) * EPI_BUF_BYTES : 0u;
+            auto make_ew = [&]() {
+                if constexpr (EP && !TR)
+                    return EpilogueWarp<OUT>{p, *epp, *em, tmD, p.out, lane, epi + (warp - 2u) * per_warp,
+                                             ptx::smem_u32(&s_in[(warp - 2u) * 2u]), &s_bias[(warp - 2u) * 128u], &s_abort};
+                else return 0;
+            };
+            [[maybe_unused]] auto ew = make_ew();
 #pragma unroll 1
-            for (uint32_t ch = krank; ch < static_cast<uint32_t>(NCH); ch += ks) {
+            for (uint32_t ch = krank + (EP ? hw * ks : 0u); ch < static_cast<uint32_t>(NCH); ch += (EP ? 2u : 1u) * ks) {
                 uint32_t own[O_CH];
                 float    acc[O_CH];
 #pragma unroll
@@ -1181,7 +1823,32 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         }
                     }
                 }
-                if constexpr (TR) {
+                if constexpr (EP && TR) {
+                    const EpilogueColumns<OUT> ec{p, *epp, lane};
+                    const uint32_t i    = ks_c.m0 + q * 32u + lane;
+                    const bool     live = (q * 32u + lane) < p.bm && i < p.M;
+                    const uint32_t col0 = ks_c.n0 + ch * 32u;
+                    const uint32_t bs   = BN < 32 ? BN : 32;
+                    const uint32_t n    = col0 < p.N ? min(min(32u, BN - ch * 32u), p.N - col0) : 0u;
+                    float          side[32];
+                    dep_wait();
+                    if (epp->streamed) ec.load_side(ks_c, col0, n, i, live, side);
+                    uint32_t (&bits)[32] = reinterpret_cast<uint32_t(&)[32]>(acc);
+                    if (n) ec.finish(ks_c, col0, n, i, live, ks_c.z_out * epp->part_blocks + col0 / bs,
+                                     ks_c.z_out * epp->part_blocks + ks_c.m0 / p.bm * 4u + q, bits, side);
+                } else if constexpr (EP) {
+                    const uint32_t col0 = ks_c.n0 + ch * O_CH;
+                    if (row_live && col0 < p.N) {
+                        dep_wait();
+                        if (epp->streamed) {
+                            ew.buffers_free();
+                            ew.request(0u, row0, col0, ks_c.z_out);
+                        }
+                        ew.prefetch_bias(ks_c, col0);
+                        __syncwarp();
+                        if (!ew.finish(ks_c, row0, col0, p.M, ew.row_bias(ks_c, row0 + lane), reinterpret_cast<const uint32_t(&)[O_CH]>(acc))) break;
+                    }
+                } else if constexpr (TR) {
                     // D(i, j) goes to out[j * M + i]: for a fixed column the warp writes 32
                     // consecutive elements (see the transposed epilogue above).
                     const uint32_t i      = ks_c.m0 + q * 32u + lane;
@@ -1229,6 +1896,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                 } // staged store
             }
             if (warp == 2 && lane == 0) B200_TL(20);
+            if constexpr (EP && !TR) ew.drain();
             if (lane == 0) ptx::tma_store_wait_read<0>();
             if (warp == 2 && lane == 0) B200_TL(21);
         }
@@ -1284,6 +1952,51 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                             const __grid_constant__ CUtensorMap tmD, const GemmParams p)
 {
     gemm_umma_body<BN, OUT, 1, TR, false, true>(tmA, tmB, &tmD, tmD, p);
+}
+
+// The GEMM with an epilogue, dense or grouped, and its form with cluster K partitions.
+template <int BN, int OUT, int CL, bool TR = false>
+__global__ void __launch_bounds__(EPI_THREADS, 1)
+    gemm_epilogue_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                         const __grid_constant__ CUtensorMap tmD, const __grid_constant__ EpilogueMaps em,
+                         const GemmParams p, const EpilogueParams ep)
+{
+    gemm_umma_body<BN, OUT, CL, TR, false, false, true>(tmA, tmB, &tmD, tmD, p, &em, &ep);
+}
+
+template <int BN, int OUT, bool TR = false>
+__global__ void __launch_bounds__(EPI_THREADS, 1)
+    gemm_epilogue_ksplit_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                                const __grid_constant__ CUtensorMap tmD, const __grid_constant__ EpilogueMaps em,
+                                const GemmParams p, const EpilogueParams ep)
+{
+    gemm_umma_body<BN, OUT, 1, TR, false, true, true>(tmA, tmB, &tmD, tmD, p, &em, &ep);
+}
+
+// Maps of a ragged-K product: group e's copies of the two operands' maps, with the row extent
+// ending at the group's end, so that the K loop's last box is zero-filled there instead of
+// reading the next group's rows.  One warp per group.
+static __global__ void __launch_bounds__(32)
+    ragged_maps_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                       CUtensorMap* __restrict__ maps, const int32_t* __restrict__ offsets, uint32_t rows)
+{
+    const uint32_t e = blockIdx.x, lane = threadIdx.x;
+    ptx::grid_dep_launch();
+    ptx::grid_dep_wait();
+    uint32_t lo, hi;
+    group_rows(offsets, e, rows, lo, hi);
+    if (lane < 16u) {
+        const uint64_t* src = reinterpret_cast<const uint64_t*>(&tmA);
+        const uint64_t* srb = reinterpret_cast<const uint64_t*>(&tmB);
+        uint64_t*       dst = reinterpret_cast<uint64_t*>(maps + 2u * e);
+        dst[lane]           = src[lane];
+        dst[16u + lane]     = srb[lane];
+    }
+    __syncwarp();
+    if (lane < 2u) {
+        ptx::tensormap_set_dim1(maps + 2u * e + lane, max(hi, 1u)); // (an extent may not be 0; such a group loads nothing)
+        ptx::fence_tensormap_release();
+    }
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -7,7 +7,7 @@
 // There is no CPU fallback: without a CUDA device every compute entry point fails.
 #include "../../include/b200_gemm.h"
 #include "gemm_kernels.cuh"
-#include "epilogue.cuh"
+#include "epilogue_kernels.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -165,6 +165,7 @@ struct DeviceCtx {
     std::atomic<bool> ready{false}; // set last, read first: initialised contexts skip the lock
     int           sm_count = 0;
     PairCache     pairs;
+    PairCache     epilogue_pairs; // of the kernels with an epilogue (tile_n up to 256 / 512)
     unsigned int* d_status = nullptr;
     // split-K workspaces, one per stream that has used split-K (calls on one stream are ordered,
     // so they can share a buffer; calls on different streams must not - and two host threads
@@ -301,6 +302,7 @@ static int get_ctx(DeviceCtx** out)
         CUDA_TRY(cudaMalloc(&c.d_status, sizeof(unsigned int)));
         CUDA_TRY(cudaMemset(c.d_status, 0, sizeof(unsigned int)));
         CUDA_TRY(set_all_kernel_attributes());
+        CUDA_TRY(set_epilogue_attributes());
         c.ready.store(true, std::memory_order_release);
     }
     *out = &c;

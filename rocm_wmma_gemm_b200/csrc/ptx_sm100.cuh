@@ -155,6 +155,24 @@ __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* tm)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
 }
 
+// Tensor maps in global memory: replacing the extent of dimension 1, making that visible, and the
+// acquire a kernel issues before its first TMA operation with such a map.
+__device__ __forceinline__ void tensormap_set_dim1(void* tm, uint32_t extent)
+{
+    asm volatile("tensormap.replace.tile.global_dim.global.b1024.b32 [%0], 1, %1;" ::"l"(reinterpret_cast<uint64_t>(tm)), "r"(extent)
+                 : "memory");
+}
+
+__device__ __forceinline__ void fence_tensormap_release()
+{
+    asm volatile("fence.proxy.tensormap::generic.release.gpu;" ::: "memory");
+}
+
+__device__ __forceinline__ void fence_tensormap_acquire(const void* tm)
+{
+    asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
+}
+
 // 3-D tiled load global -> this CTA's shared memory, completion on this CTA's mbarrier.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tm, uint32_t bar,
                                             int32_t c0, int32_t c1, int32_t c2, uint64_t policy)
