@@ -35,7 +35,8 @@ struct EpilogueParams {
     float*         part;        // gradient: nullptr or partial bias gradients [batch][part_blocks][length]
     uint64_t       bias_stride; // elements between the biases of consecutive batch items / groups
     uint32_t       act;
-    float          c0, c1;      // ACT_SIGMOID
+    float          k0, k1;      // ACT_SIGMOID: -c0 log2(e), -c1 log2(e)
+    float          slope0, slope1; // ACT_SIGMOID: c0, 3 c1
     uint32_t       gradient;
     uint32_t       part_blocks; // blocks per batch item (all groups together)
     uint32_t       part_rows;   // rows of the caller's C per block
@@ -52,32 +53,92 @@ struct EpilogueParams {
     const CUtensorMap* maps;         // ragged K: two maps per group, their row extents ending at the group's end
 };
 
-// sigmoid in f32: e^-s overflows to infinity and its reciprocal to 0 far left, which is right.
-__device__ __forceinline__ float sigmoid_f32(float s) { return __fdividef(1.f, 1.f + __expf(-s)); }
-
-// (a NaN stays a NaN under every activation)
-template <uint32_t ACT>
-__device__ __forceinline__ float act_value(float x, float c0, float c1)
+// Two elements at a time: the packed f32 instructions halve the issue slots of everything but the
+// special functions.
+__device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float  ex2(float x)
 {
-    if constexpr (ACT == ACT_RELU) return x < 0.f ? 0.f : x;
-    else if constexpr (ACT == ACT_SIGMOID) return x * sigmoid_f32(x * fmaf(c1 * x, x, c0));
-    else if constexpr (ACT == ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678f));
-    else return x;
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float2 ex2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
+__device__ __forceinline__ float2 rcp(float2 x) { return make_float2(rcp(x.x), rcp(x.y)); }
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// sigmoid(x (c0 + c1 x^2)) for k0 = -c0 log2(e), k1 = -c1 log2(e); x2 = x^2.  Far left 2^s overflows to
+// infinity and its reciprocal is 0, which is right.
+__device__ __forceinline__ float2 sigmoid_of(float2 x, float2 x2, float k0, float k1)
+{
+    const float2 s = __fmul2_rn(x, __ffma2_rn(x2, splat(k1), splat(k0)));
+    return rcp(__fadd2_rn(ex2(s), splat(1.f)));
 }
 
-template <uint32_t ACT>
-__device__ __forceinline__ float act_slope(float x, float c0, float c1)
+// Normal distribution: tail = 1 - Phi(|x|) and e = exp(-x^2 / 2), which the density shares.  The tail is
+// e / 2 times a polynomial in t = 1 / (1 + 0.3275911 |x| / sqrt 2): Abramowitz and Stegun 7.1.26, erf
+// within 1.5e-7; in f32 the tail is within 3e-7.
+__device__ __forceinline__ void normal_tail(float2 x, float2 x2, float2& tail, float2& e)
 {
-    if constexpr (ACT == ACT_RELU) return x > 0.f ? 1.f : (x <= 0.f ? 0.f : x);
-    else if constexpr (ACT == ACT_SIGMOID) {
-        // d/dx x s(u(x)) = s + x s (1 - s) u'(x),  u = c0 x + c1 x^3
-        const float x2 = x * x;
-        const float s  = sigmoid_f32(x * fmaf(c1, x2, c0));
-        return fmaf(x * s * (1.f - s), fmaf(3.f * c1, x2, c0), s);
+    const float2 t = rcp(make_float2(fmaf(fabsf(x.x), 0.23164190f, 1.f), fmaf(fabsf(x.y), 0.23164190f, 1.f)));
+    e              = ex2(__fmul2_rn(x2, splat(-0.5f * LOG2E)));
+    float2 q       = __ffma2_rn(t, splat(0.5f * 1.061405429f), splat(0.5f * -1.453152027f));
+    q              = __ffma2_rn(q, t, splat(0.5f * 1.421413741f));
+    q              = __ffma2_rn(q, t, splat(0.5f * -0.284496736f));
+    q              = __ffma2_rn(q, t, splat(0.5f * 0.254829592f));
+    tail           = __fmul2_rn(__fmul2_rn(q, t), e);
+}
+
+// The activation and its slope.  (A NaN stays a NaN under every activation.)
+template <uint32_t ACT>
+__device__ __forceinline__ float2 act_value(float2 x, const EpilogueParams& ep)
+{
+    if constexpr (ACT == ACT_RELU) {
+        return make_float2(x.x < 0.f ? 0.f : x.x, x.y < 0.f ? 0.f : x.y);
+    } else if constexpr (ACT == ACT_SIGMOID) {
+        return __fmul2_rn(x, sigmoid_of(x, __fmul2_rn(x, x), ep.k0, ep.k1));
     } else if constexpr (ACT == ACT_GELU) {
-        return fmaf(x * 0.39894228f, __expf(-0.5f * x * x), 0.5f * (1.f + erff(x * 0.70710678f)));
-    } else return 1.f;
+        float2 tail, e;
+        normal_tail(x, __fmul2_rn(x, x), tail, e);
+        const float2 y = __fmul2_rn(x, tail); // x Phi(x) = x tail on the left, x - x tail on the right
+        return make_float2(x.x > 0.f ? x.x - y.x : y.x, x.y > 0.f ? x.y - y.y : y.y);
+    } else {
+        return x;
+    }
 }
+
+template <uint32_t ACT>
+__device__ __forceinline__ float2 act_slope(float2 x, const EpilogueParams& ep)
+{
+    if constexpr (ACT == ACT_RELU) {
+        return make_float2(x.x > 0.f ? 1.f : (x.x <= 0.f ? 0.f : x.x), x.y > 0.f ? 1.f : (x.y <= 0.f ? 0.f : x.y));
+    } else if constexpr (ACT == ACT_SIGMOID) {
+        // d/dx x s(u(x)) = s + x s (1 - s) u'(x),  u = c0 x + c1 x^3
+        const float2 x2 = __fmul2_rn(x, x);
+        const float2 s  = sigmoid_of(x, x2, ep.k0, ep.k1);
+        const float2 w  = __fmul2_rn(__fmul2_rn(x, s), __ffma2_rn(s, splat(-1.f), splat(1.f)));
+        return __ffma2_rn(w, __ffma2_rn(x2, splat(ep.slope1), splat(ep.slope0)), s);
+    } else if constexpr (ACT == ACT_GELU) {
+        float2 tail, e;
+        normal_tail(x, __fmul2_rn(x, x), tail, e);
+        const float2 phi = make_float2(x.x > 0.f ? 1.f - tail.x : tail.x, x.y > 0.f ? 1.f - tail.y : tail.y);
+        return __ffma2_rn(__fmul2_rn(x, splat(0.39894228f)), e, phi);
+    } else {
+        return splat(1.f);
+    }
+}
+
+// One element.
+template <uint32_t ACT>
+__device__ __forceinline__ float act_value(float x, const EpilogueParams& ep) { return act_value<ACT>(splat(x), ep).x; }
+template <uint32_t ACT>
+__device__ __forceinline__ float act_slope(float x, const EpilogueParams& ep) { return act_slope<ACT>(splat(x), ep).x; }
 
 // Calls f with the activation as a compile-time constant (the loop over a tile's elements is
 // inside f, so the choice is made once per chunk).
@@ -146,7 +207,7 @@ __device__ __forceinline__ uint32_t group_first_block(uint32_t first_row, uint32
 
 // The group and rows of row-tile number `want` (tiles of `tile` rows, groups in order); the whole
 // warp takes part.  False when there are fewer tiles.
-__device__ __forceinline__ bool locate_row_tile(const int32_t* __restrict__ offsets, uint32_t groups, uint32_t rows,
+__device__ __forceinline__ bool locate_row_tile(const int32_t* offsets, uint32_t groups, uint32_t rows,
                                                 uint32_t tile, uint32_t want, uint32_t& e, uint32_t& first,
                                                 uint32_t& row0, uint32_t& row1)
 {
@@ -154,8 +215,8 @@ __device__ __forceinline__ bool locate_row_tile(const int32_t* __restrict__ offs
     uint32_t       top = 0u, before = 0u; // running maximum of the offsets, tiles of the groups so far
     for (uint32_t g0 = 0; g0 < groups; g0 += 32u) {
         const uint32_t g  = g0 + lane;
-        uint32_t       lo = g < groups ? clamp_offset(__ldg(offsets + g), rows) : 0u;
-        uint32_t       hi = g < groups ? clamp_offset(__ldg(offsets + g + 1u), rows) : 0u;
+        uint32_t       lo = g < groups ? clamp_offset(offsets[g], rows) : 0u;
+        uint32_t       hi = g < groups ? clamp_offset(offsets[g + 1u], rows) : 0u;
         lo = max(warp_scan_max(lo, lane), top);
         hi = max(warp_scan_max(hi, lane), lo);
         const uint32_t tiles = g < groups ? (hi - lo + tile - 1u) / tile : 0u;
@@ -178,16 +239,16 @@ __device__ __forceinline__ bool locate_row_tile(const int32_t* __restrict__ offs
 }
 
 // Rows [lo, hi) of group e; the whole warp takes part.
-__device__ __forceinline__ void group_rows(const int32_t* __restrict__ offsets, uint32_t e, uint32_t rows, uint32_t& lo,
+__device__ __forceinline__ void group_rows(const int32_t* offsets, uint32_t e, uint32_t rows, uint32_t& lo,
                                            uint32_t& hi)
 {
     const uint32_t lane = threadIdx.x & 31u;
     uint32_t       top  = 0u;
-    for (uint32_t g = lane; g <= e; g += 32u) top = max(top, clamp_offset(__ldg(offsets + g), rows));
+    for (uint32_t g = lane; g <= e; g += 32u) top = max(top, clamp_offset(offsets[g], rows));
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
     lo = top;
-    hi = max(lo, clamp_offset(__ldg(offsets + e + 1u), rows));
+    hi = max(lo, clamp_offset(offsets[e + 1u], rows));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -294,11 +355,11 @@ __global__ void __launch_bounds__(256) simple_product_kernel(const SimpleParams 
                     const uint64_t at = m * p.c_sm + n * p.c_sn;
                     float          v  = acc[i][j];
                     if (ep.gradient) {
-                        if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(pre[at]), ep.c0, ep.c1));
+                        if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(pre[at]), ep));
                     } else {
                         if (bias) v += to_f32(bias[z * ep.bias_stride + n]);
                         if (pre) pre[at] = from_f32<TOut>(v);
-                        v = act_value<ACT>(v, ep.c0, ep.c1);
+                        v = act_value<ACT>(v, ep);
                         if (res) v += to_f32(res[at]);
                     }
                     C[at]     = from_f32<TOut>(v);
@@ -332,8 +393,8 @@ __global__ void __launch_bounds__(256) simple_product_kernel(const SimpleParams 
 constexpr uint32_t SUM_LANES = 16;
 
 static __global__ void __launch_bounds__(32 * SUM_LANES)
-    bias_grad_sum_kernel(const float* __restrict__ part, float* __restrict__ out, uint32_t length, uint64_t out_stride,
-                         uint64_t blocks, const int32_t* __restrict__ offsets, uint32_t rows, uint32_t part_rows)
+    bias_grad_sum_kernel(const float* part, float* out, uint32_t length, uint64_t out_stride,
+                         uint64_t blocks, const int32_t* offsets, uint32_t rows, uint32_t part_rows)
 {
     __shared__ float s_sum[SUM_LANES][32];
     const uint32_t tx = threadIdx.x & 31u, ty = threadIdx.x >> 5, n = blockIdx.x * 32u + tx;
@@ -349,7 +410,7 @@ static __global__ void __launch_bounds__(32 * SUM_LANES)
     float s = 0.f;
     if (n < length)
 #pragma unroll 4
-        for (uint64_t b = ty; b < count; b += SUM_LANES) s += __ldg(part + (b0 + b) * length + n);
+        for (uint64_t b = ty; b < count; b += SUM_LANES) s += part[(b0 + b) * length + n];
     s_sum[ty][tx] = s;
     __syncthreads();
     if (ty == 0 && n < length) {
@@ -435,14 +496,14 @@ __global__ void __launch_bounds__(256) act_backward_rows_kernel(const ActBackwar
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         float v = g.get(i);
-                        if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(x.get(i), ep.c0, ep.c1));
+                        if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(x.get(i), ep));
                         o.set(i, v);
                         sum[i] += v;
                     }
                     if (dz) *reinterpret_cast<uint4*>(dz + at) = o.raw;
                 } else {
                     float v = to_f32(dy[at]);
-                    if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(z[at]), ep.c0, ep.c1));
+                    if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(z[at]), ep));
                     if (dz) dz[at] = from_f32<T>(v);
                     sum[0] += v;
                 }
@@ -487,14 +548,14 @@ __global__ void __launch_bounds__(256) act_backward_cols_kernel(const ActBackwar
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     float v = g.get(i);
-                    if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(x.get(i), ep.c0, ep.c1));
+                    if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(x.get(i), ep));
                     o.set(i, v);
                     sum += v;
                 }
                 if (dz) *reinterpret_cast<uint4*>(dz + i0) = o.raw;
             } else {
                 float v = to_f32(dy[i0]);
-                if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(z[i0]), ep.c0, ep.c1));
+                if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(z[i0]), ep));
                 if (dz) dz[i0] = from_f32<T>(v);
                 sum += v;
             }

@@ -127,6 +127,7 @@ constexpr int      MAX_STAGES     = 12; // ring depth of the staged-epilogue ker
 constexpr int      MAX_SLAB_STAGES = 24; // ring depth of the transposed-epilogue (slab) kernels
 constexpr int      GEMM_THREADS   = 192; // warp 0 TMA, warp 1 MMA, warps 2..5 epilogue
 constexpr int      EPI_WARPS      = 8;   // kernels with an epilogue (activation ...): warps 2..9, two per TMEM lane quarter
+constexpr int      EPI_SETS       = EPI_WARPS / 4; // warps that share a lane quarter: they take its column chunks in turn
 constexpr int      EPI_THREADS    = 64 + 32 * EPI_WARPS;
 constexpr uint32_t A_TILE_BYTES   = BLOCK_M * BLOCK_K * 2;
 constexpr uint32_t EPI_BUF_BYTES  = 32 * 128; // one warp's 32 rows x 128 B
@@ -401,7 +402,7 @@ __device__ __forceinline__ void build_group_table(const EpilogueParams& ep, uint
     uint32_t       top = 0u, before = 0u;
     for (uint32_t g0 = 0; g0 <= ep.groups; g0 += 32u) {
         const uint32_t g = g0 + lane;
-        const uint32_t v = g <= ep.groups ? clamp_offset(__ldg(ep.offsets + g), ep.rows) : 0u;
+        const uint32_t v = g <= ep.groups ? clamp_offset(ep.offsets[g], ep.rows) : 0u;
         const uint32_t m = max(warp_scan_max(v, lane), top); // first row of group g
         uint32_t       prev = __shfl_up_sync(0xffffffffu, m, 1);
         if (lane == 0) prev = g0 ? top : m;
@@ -576,11 +577,12 @@ struct EpilogueMaps {
     CUtensorMap in, aux;
 };
 
-// Sum of v[j] over the 32 lanes, for 32 values of j: lane j receives the sum of v[j].
-__device__ __forceinline__ float warp_column_sums(float (&v)[32], uint32_t lane)
+// Sum of v[j] over the 32 lanes, for N = 16 or 32 values of j: lane l receives the sum of v[l % N].
+template <int N>
+__device__ __forceinline__ float warp_column_sums(float (&v)[N], uint32_t lane)
 {
 #pragma unroll
-    for (int s = 16; s > 0; s /= 2) {
+    for (int s = N / 2; s > 0; s /= 2) {
         const bool up = (lane & s) != 0u;
 #pragma unroll
         for (int i = 0; i < s; ++i) {
@@ -589,7 +591,114 @@ __device__ __forceinline__ float warp_column_sums(float (&v)[32], uint32_t lane)
             v[i]             = keep + __shfl_xor_sync(0xffffffffu, send, s);
         }
     }
-    return v[0];
+    if constexpr (N == 16) return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
+    else return v[0];
+}
+
+// The epilogues work in pieces of 32 columns (16 where the accumulator is read transposed), in
+// loops that are not unrolled: the whole of a piece - bias, activation, residual, conversion - is a few
+// hundred instructions, which stay in the instruction cache.
+constexpr int PIECE = 32, COLUMN_PIECE = 16;
+
+template <int N>
+__device__ __forceinline__ void tmem_ld_piece(uint32_t addr, uint32_t (&r)[N])
+{
+    if constexpr (N == 32) ptx::tmem_ld_32x32(addr, r);
+    else ptx::tmem_ld_32x16(addr, r);
+}
+
+// Accumulator columns from TMEM.  The load and its wait stay together: a load in flight across a
+// branch or a loop's back edge would let the compiler copy its destination registers, and reuse
+// them, before the hardware has written them.
+template <int N>
+struct TmemPieces {
+    uint32_t addr;  // first column of the chunk
+    uint32_t count; // pieces
+    bool     empty; // nothing was accumulated: zeros
+
+    // Piece i (in order); `done` is called once the chunk's last piece has been read.
+    template <class F>
+    __device__ __forceinline__ void get(uint32_t i, float (&v)[N], F&& done)
+    {
+        uint32_t t[N];
+        tmem_ld_piece(addr + i * N, t);
+        ptx::tmem_ld_wait(t);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = empty ? 0.f : __uint_as_float(t[j]);
+        if (i + 1u == count) done();
+    }
+};
+
+// Sums of a cluster's K partitions: this CTA's own part from TMEM, the others' from shared memory
+// (laid out [16-byte unit][lane], see the cluster exchange), added in partition order.
+template <int N>
+struct ClusterPieces {
+    uint32_t addr;       // this CTA's accumulator columns of the chunk
+    uint32_t ring;       // partial of partition 0 of this chunk, this warp's rows, this lane
+    uint32_t slot_bytes; // from one partition's to the next
+    uint32_t parts, rank;
+
+    template <class F>
+    __device__ __forceinline__ void get(uint32_t i, float (&v)[N], F&&) const
+    {
+        uint32_t own[N];
+        tmem_ld_piece(addr + i * N, own);
+        ptx::tmem_ld_wait(own);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = 0.f;
+#pragma unroll 1
+        for (uint32_t s = 0; s < parts; ++s) {
+            if (s == rank) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] += __uint_as_float(own[j]);
+            } else {
+#pragma unroll
+                for (uint32_t u = 0; u < N / 4; ++u) {
+                    uint32_t x[4];
+                    ptx::ld_shared_v4(ring + s * slot_bytes + (i * (N / 4) + u) * 512u, x[0], x[1], x[2], x[3]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[4 * u + k] += __uint_as_float(x[k]);
+                }
+            }
+        }
+    }
+};
+
+// Element-wise steps of an epilogue over N values.
+template <int N>
+__device__ __forceinline__ void apply_activation(const EpilogueParams& ep, float (&v)[N])
+{
+    with_act(ep.act, [&](auto tag) {
+        constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const float2 y = act_value<ACT>(make_float2(v[j], v[j + 1]), ep);
+            v[j] = y.x, v[j + 1] = y.y;
+        }
+    });
+}
+
+template <int N>
+__device__ __forceinline__ void apply_slope(const EpilogueParams& ep, float (&v)[N], const float (&z)[N])
+{
+    with_act(ep.act, [&](auto tag) {
+        constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const float2 y = __fmul2_rn(make_float2(v[j], v[j + 1]), act_slope<ACT>(make_float2(z[j], z[j + 1]), ep));
+            v[j] = y.x, v[j + 1] = y.y;
+        }
+    });
+}
+
+template <int N>
+__device__ __forceinline__ void add_values(float* v, const float (&t)[N])
+{
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        const float2 y = __fadd2_rn(make_float2(v[j], v[j + 1]), make_float2(t[j], t[j + 1]));
+        v[j] = y.x, v[j + 1] = y.y;
+    }
 }
 
 template <int OUT>
@@ -621,6 +730,10 @@ __device__ __forceinline__ void pack16(const float* v, uint32_t (&w)[4])
         else w[k] = pack2<OUT>(__float_as_uint(v[2 * k]), __float_as_uint(v[2 * k + 1]));
     }
 }
+
+// (Operands that may be absent - bias, the read matrix, offsets - are read with ordinary loads.  A
+// load through the read-only path counts as safe to execute early: with no bias, the compiler moved
+// `__ldg(bias + i)` out of a loop and above the test of the pointer.)
 
 // One epilogue warp of a staged kernel with an epilogue: 32 rows x 128-byte column chunks.
 template <int OUT>
@@ -674,14 +787,14 @@ struct EpilogueWarp {
 #pragma unroll
         for (int h = 0; h < PARTS; ++h) {
             const uint32_t col = col0 + h * 32u + lane;
-            bias_reg[h]        = col < p.N ? __ldg(b + col) : from_f32<T>(0.f);
+            bias_reg[h]        = col < p.N ? b[col] : from_f32<T>(0.f);
         }
     }
 
     __device__ __forceinline__ float row_bias(const WorkCoord& c, uint32_t row) const
     {
         if (!ep.bias || !ep.bias_on_rows || row >= p.M) return 0.f;
-        return to_f32(__ldg(static_cast<const T*>(ep.bias) + c.z_in * ep.bias_stride + row));
+        return to_f32(static_cast<const T*>(ep.bias)[c.z_in * ep.bias_stride + row]);
     }
 
     __device__ __forceinline__ void store_row_from(uint32_t rowaddr, void* base, uint32_t row, uint32_t col0) const
@@ -697,8 +810,9 @@ struct EpilogueWarp {
     }
 
     // The chunk at (row0, col0) from its accumulators; `end` bounds the rows.  False: a wait ran out.
+    template <class Pieces, class F>
     __device__ __forceinline__ bool finish(const WorkCoord& c, uint32_t row0, uint32_t col0, uint32_t end, float bias_row,
-                                           const uint32_t (&a)[CH])
+                                           Pieces& pieces, F&& accumulators_read)
     {
         const uint32_t b    = slot(0);
         const uint32_t sbuf = stg + b * EPI_BUF_BYTES, rowaddr = sbuf + lane * 128u;
@@ -723,29 +837,22 @@ struct EpilogueWarp {
         }
         __syncwarp();
         float row_sum = 0.f;
-#pragma unroll
-        for (int h = 0; h < PARTS; ++h) {
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(a[h * 32 + j]);
-            // 16-byte unit i of this half's columns within the row's 128 bytes (128-byte swizzle)
-            constexpr uint32_t UNITS = 32 / UNIT;
-            auto at = [&](uint32_t i) { return ((h * UNITS + i) ^ (lane & 7u)) << 4; };
+#pragma unroll 1
+        for (uint32_t pc = 0; pc < CH / PIECE; ++pc) {
+            constexpr uint32_t UNITS = PIECE / UNIT; // 16-byte units of a row's piece
+            auto  at = [&](uint32_t i) { return ((pc * UNITS + i) ^ (lane & 7u)) << 4; }; // (128-byte swizzle)
+            float v[PIECE];
+            pieces.get(pc, v, accumulators_read);
             if (ep.gradient) {
                 if (ep.streamed) {
-                    with_act(ep.act, [&](auto tag) {
-                        constexpr uint32_t ACT = decltype(tag)::value;
+                    float z[PIECE];
 #pragma unroll
-                        for (uint32_t i = 0; i < UNITS; ++i) {
-                            uint32_t w[4];
-                            float    z[UNIT];
-                            ptx::ld_shared_v4(rowaddr + at(i), w[0], w[1], w[2], w[3]);
-                            unpack16<OUT>(w, z);
-#pragma unroll
-                            for (uint32_t j = 0; j < UNIT; ++j)
-                                v[i * UNIT + j] = __fmul_rn(v[i * UNIT + j], act_slope<ACT>(z[j], ep.c0, ep.c1));
-                        }
-                    });
+                    for (uint32_t i = 0; i < UNITS; ++i) {
+                        uint32_t w[4];
+                        ptx::ld_shared_v4(rowaddr + at(i), w[0], w[1], w[2], w[3]);
+                        unpack16<OUT>(w, z + i * UNIT);
+                    }
+                    apply_slope(ep, v, z);
                 }
             } else {
                 if (col_bias) {
@@ -753,14 +860,13 @@ struct EpilogueWarp {
                     for (uint32_t i = 0; i < UNITS; ++i) {
                         uint32_t w[4];
                         float    t[UNIT];
-                        ptx::ld_shared_v4(ptx::smem_u32(bias_sm) + (h * UNITS + i) * 16u, w[0], w[1], w[2], w[3]);
+                        ptx::ld_shared_v4(ptx::smem_u32(bias_sm) + (pc * UNITS + i) * 16u, w[0], w[1], w[2], w[3]);
                         unpack16<OUT>(w, t);
-#pragma unroll
-                        for (uint32_t j = 0; j < UNIT; ++j) v[i * UNIT + j] += t[j];
+                        add_values(v + i * UNIT, t);
                     }
                 } else if (ep.bias) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] += bias_row;
+                    for (int j = 0; j < PIECE; ++j) v[j] += bias_row;
                 }
                 if (ep.aux) {
 #pragma unroll
@@ -770,11 +876,7 @@ struct EpilogueWarp {
                         st_shared_v4(xrow + at(i), w[0], w[1], w[2], w[3]);
                     }
                 }
-                with_act(ep.act, [&](auto tag) {
-                    constexpr uint32_t ACT = decltype(tag)::value;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = act_value<ACT>(v[j], ep.c0, ep.c1);
-                });
+                apply_activation(ep, v);
                 if (ep.streamed) {
 #pragma unroll
                     for (uint32_t i = 0; i < UNITS; ++i) {
@@ -782,8 +884,7 @@ struct EpilogueWarp {
                         float    r[UNIT];
                         ptx::ld_shared_v4(rowaddr + at(i), w[0], w[1], w[2], w[3]);
                         unpack16<OUT>(w, r);
-#pragma unroll
-                        for (uint32_t j = 0; j < UNIT; ++j) v[i * UNIT + j] += r[j];
+                        add_values(v + i * UNIT, r);
                     }
                 }
             }
@@ -795,18 +896,18 @@ struct EpilogueWarp {
             }
             if (ep.part) {
                 // (what lies outside C may be NaN: a zero-filled operand times an infinity)
+                const uint32_t pcol = col0 + pc * PIECE;
                 if (ep.bias_on_rows) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) row_sum += col0 + h * 32 + j < p.N ? v[j] : 0.f;
+                    for (int j = 0; j < PIECE; ++j) row_sum += pcol + j < p.N ? v[j] : 0.f;
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = row < end ? v[j] : 0.f;
+                    for (int j = 0; j < PIECE; ++j) v[j] = row < end ? v[j] : 0.f;
                     const float    sum   = warp_column_sums(v, lane);
                     const uint32_t block = ep.ragged == RAGGED_ROWS
                                                ? group_first_block(c.first, c.group, 32u) + (row0 - c.first) / 32u
                                                : c.z_out * ep.part_blocks + row0 / 32u;
-                    const uint32_t col   = col0 + h * 32u + lane;
-                    if (col < p.N) ep.part[static_cast<uint64_t>(block) * p.N + col] = sum;
+                    if (lane < PIECE && pcol + lane < p.N) ep.part[static_cast<uint64_t>(block) * p.N + pcol + lane] = sum;
                 }
             }
         }
@@ -848,8 +949,8 @@ struct EpilogueWarp {
     }
 };
 
-// The transposing epilogue's part of a tile with an epilogue: `n` <= 32 columns from col0 on of
-// kernel row i (this lane's), D(i, j) lying at out[j * M + i].  `side`: the read matrix's values.
+// The transposing epilogue's part of a tile with an epilogue: a piece of `n` <= 16 columns from col0
+// on of kernel row i (this lane's), D(i, j) lying at out[j * M + i].  `side`: the read matrix's values.
 template <int OUT>
 struct EpilogueColumns {
     using T = OutType<OUT>;
@@ -862,73 +963,76 @@ struct EpilogueColumns {
         return (static_cast<uint64_t>(c.z_out) * p.N + col) * p.M + i;
     }
 
-    __device__ __forceinline__ void load_side(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, float (&side)[32]) const
+    __device__ __forceinline__ void load_side(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, float (&side)[COLUMN_PIECE]) const
     {
         const T* src = static_cast<const T*>(ep.gradient ? ep.preact : ep.residual);
 #pragma unroll
-        for (uint32_t r = 0; r < 32; ++r) side[r] = live && r < n ? to_f32(src[at(c, col0 + r, i)]) : 0.f;
+        for (uint32_t r = 0; r < COLUMN_PIECE; ++r) side[r] = live && r < n ? to_f32(src[at(c, col0 + r, i)]) : 0.f;
     }
 
-    // `block`: where a sum along the columns goes; `block_rows`: where sums over the rows go.
-    __device__ __forceinline__ void finish(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, uint32_t block,
-                                           uint32_t block_rows, const uint32_t (&a)[32], const float (&side)[32]) const
+    // Bias gradients: the piece's sum over the columns is added to `row_sum`, its sums over the rows go
+    // to row `block_rows` of the partial sums.
+    __device__ __forceinline__ void finish(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, uint32_t block_rows,
+                                           float (&v)[COLUMN_PIECE], const float (&side)[COLUMN_PIECE], float& row_sum) const
     {
-        float v[32];
-#pragma unroll
-        for (int r = 0; r < 32; ++r) v[r] = __uint_as_float(a[r]);
         if (ep.gradient) {
             if (ep.streamed)
-                with_act(ep.act, [&](auto tag) {
-                    constexpr uint32_t ACT = decltype(tag)::value;
-#pragma unroll
-                    for (int r = 0; r < 32; ++r) v[r] = __fmul_rn(v[r], act_slope<ACT>(side[r], ep.c0, ep.c1));
-                });
+                apply_slope(ep, v, side);
         } else {
             if (ep.bias) {
                 const T* bias = static_cast<const T*>(ep.bias) + (ep.ragged == RAGGED_ROWS ? c.group : c.z_in) * ep.bias_stride;
                 if (ep.bias_on_rows) {
-                    const float b = live ? to_f32(__ldg(bias + i)) : 0.f;
+                    const float b = live ? to_f32(bias[i]) : 0.f;
 #pragma unroll
-                    for (int r = 0; r < 32; ++r) v[r] += b;
+                    for (int r = 0; r < COLUMN_PIECE; ++r) v[r] += b;
                 } else {
 #pragma unroll
-                    for (uint32_t r = 0; r < 32; ++r) v[r] += r < n ? to_f32(__ldg(bias + col0 + r)) : 0.f;
+                    for (uint32_t r = 0; r < COLUMN_PIECE; ++r) v[r] += r < n ? to_f32(bias[col0 + r]) : 0.f;
                 }
             }
             if (ep.aux && live) {
                 T* pre = static_cast<T*>(ep.preact);
 #pragma unroll
-                for (uint32_t r = 0; r < 32; ++r)
+                for (uint32_t r = 0; r < COLUMN_PIECE; ++r)
                     if (r < n) pre[at(c, col0 + r, i)] = from_f32<T>(v[r]);
             }
-            with_act(ep.act, [&](auto tag) {
-                constexpr uint32_t ACT = decltype(tag)::value;
-#pragma unroll
-                for (int r = 0; r < 32; ++r) v[r] = act_value<ACT>(v[r], ep.c0, ep.c1);
-            });
-            if (ep.streamed) {
-#pragma unroll
-                for (int r = 0; r < 32; ++r) v[r] += side[r];
-            }
+            apply_activation(ep, v);
+            if (ep.streamed) add_values(v, side);
         }
         if (live) {
             T* out = static_cast<T*>(p.out);
 #pragma unroll
-            for (uint32_t r = 0; r < 32; ++r)
+            for (uint32_t r = 0; r < COLUMN_PIECE; ++r)
                 if (r < n) out[at(c, col0 + r, i)] = from_f32<T>(v[r]);
         }
         if (!ep.part) return;
         if (ep.bias_on_rows) {
-            float sum = 0.f;
 #pragma unroll
-            for (uint32_t r = 0; r < 32; ++r) sum += r < n ? v[r] : 0.f;
-            if (live) ep.part[static_cast<uint64_t>(block) * p.M + i] = sum;
+            for (uint32_t r = 0; r < COLUMN_PIECE; ++r) row_sum += r < n ? v[r] : 0.f;
         } else {
 #pragma unroll
-            for (int r = 0; r < 32; ++r) v[r] = live ? v[r] : 0.f;
+            for (int r = 0; r < COLUMN_PIECE; ++r) v[r] = live ? v[r] : 0.f;
             const float sum = warp_column_sums(v, lane);
             if (lane < n) ep.part[static_cast<uint64_t>(block_rows) * p.N + col0 + lane] = sum;
         }
+    }
+
+    // A chunk of up to 32 columns from col0 on, `n` of them live.  `side`: the read values of the first
+    // piece, loaded before the accumulator was awaited.
+    template <class Pieces, class F>
+    __device__ __forceinline__ void chunk(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, uint32_t block,
+                                          uint32_t block_rows, Pieces& pieces, uint32_t npieces, float (&side)[COLUMN_PIECE], F&& accumulators_read) const
+    {
+        float row_sum = 0.f;
+#pragma unroll 1
+        for (uint32_t pc = 0; pc < npieces; ++pc) {
+            const uint32_t m = n > pc * COLUMN_PIECE ? min(n - pc * COLUMN_PIECE, static_cast<uint32_t>(COLUMN_PIECE)) : 0u;
+            float          v[COLUMN_PIECE];
+            if (pc > 0u && ep.streamed) load_side(c, col0 + pc * COLUMN_PIECE, m, i, live, side);
+            pieces.get(pc, v, accumulators_read);
+            if (m) finish(c, col0 + pc * COLUMN_PIECE, m, i, live, block_rows, v, side, row_sum);
+        }
+        if (ep.part && ep.bias_on_rows && live && n) ep.part[static_cast<uint64_t>(block) * p.M + i] = row_sum;
     }
 };
 
@@ -1419,7 +1523,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
     } else if constexpr (EP) {
         // ------------------------------------------------------------------ epilogue with activation, bias, ...
         const uint32_t q  = warp & 3u;          // TMEM lane quarter this warp may read
-        const uint32_t hw = (warp - 2u) >> 2;   // takes column chunks hw, hw + 2, ...
+        const uint32_t hw = (warp - 2u) >> 2;   // takes column chunks hw, hw + EPI_SETS, ...
         uint32_t       it = 0;
         bool           ok = true;
         WorkCursor     cur = work_begin(p, unit, krank);
@@ -1457,25 +1561,23 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                 bool           seen = false;
                 dep_wait();
 #pragma unroll 1
-                for (uint32_t ch = hw; ch < CHUNKS; ch += 2u) {
+                for (uint32_t ch = hw; ch < CHUNKS; ch += EPI_SETS) {
                     const uint32_t col0 = c.n0 + ch * 32u;
                     const uint32_t n    = col0 < c.end ? min(min(32u, BN - ch * 32u), c.end - col0) : 0u;
-                    float          side[32];
-                    if (epp->streamed) ec.load_side(c, col0, n, i, live, side);
+                    constexpr uint32_t NP = (BN < 32 ? BN : 32) / COLUMN_PIECE; // pieces of a chunk
+                    float          side[COLUMN_PIECE];
+                    if (epp->streamed) ec.load_side(c, col0, min(n, static_cast<uint32_t>(COLUMN_PIECE)), i, live, side);
                     if (!seen) {
                         ok = accumulator(buf, (it / NUM_ACC) & 1u);
                         if (!ok) break;
                         seen = true;
                     }
-                    uint32_t v[32];
-                    ptx::tmem_ld_32x32(tacc + ch * 32u, v);
-                    ptx::tmem_ld_wait(v);
-                    if (ch + 2u >= CHUNKS) release(buf);
-                    if (n == 0u) continue;
+                    TmemPieces<COLUMN_PIECE> pieces{tacc + ch * 32u, NP, false};
                     const uint32_t block = epp->ragged == RAGGED_ROWS
                                                ? group_first_block(c.first, c.group, bs) + (col0 - c.first) / bs
                                                : c.z_out * epp->part_blocks + col0 / bs;
-                    ec.finish(c, col0, n, i, live, block, c.z_out * epp->part_blocks + c.m0 / p.bm * 4u + q, v, side);
+                    ec.chunk(c, col0, n, i, live, block, c.z_out * epp->part_blocks + c.m0 / p.bm * 4u + q, pieces, NP, side,
+                             [&] { if (ch + EPI_SETS >= CHUNKS) release(buf); });
                 }
                 if (ok && !seen) { // fewer chunks than warps
                     ok = accumulator(buf, (it / NUM_ACC) & 1u);
@@ -1497,8 +1599,8 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                     const uint32_t row0   = c.m0 + rank * BLOCK_M + q * 32u;
                     const uint32_t width  = FLEX ? wn : static_cast<uint32_t>(UMMA_N);
                     const uint32_t live   = (row0 < c.end && q * 32u < p.bm && colh < p.N) ? (min(width, p.N - colh) + EW::CH - 1u) / EW::CH : 0u;
-                    const uint32_t mine   = live > hw ? (live - hw + 1u) / 2u : 0u; // this warp's chunks: hw, hw + 2, ...
-                    auto           col    = [&](uint32_t k) { return colh + (hw + 2u * k) * EW::CH; };
+                    const uint32_t mine   = live > hw ? (live - hw + EPI_SETS - 1u) / EPI_SETS : 0u; // this warp's chunks: hw, hw + EPI_SETS, ...
+                    auto           col    = [&](uint32_t k) { return colh + (hw + EPI_SETS * k) * EW::CH; };
                     const uint32_t tacc   = tmem_base + ((q * 32u) << 16) + (NSUB == 2 ? hh * UMMA_N : buf * ACC_COLS);
                     float          bias_row = 0.f;
                     if (mine) {
@@ -1515,29 +1617,13 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                     if (mine == 0u) release(bar_i);
 #pragma unroll 1
                     for (uint32_t k = 0; k < mine; ++k) {
-                        uint32_t a[EW::CH];
-                        if (c.kb1 > c.kb0) {
-                            uint32_t (&a0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&a[0]);
-                            ptx::tmem_ld_32x32(tacc + (hw + 2u * k) * EW::CH, a0);
-                            if constexpr (EW::CH == 64) {
-                                uint32_t (&a1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&a[32]);
-                                ptx::tmem_ld_32x32(tacc + (hw + 2u * k) * EW::CH + 32u, a1);
-                                ptx::tmem_ld_wait(a0);
-                                ptx::tmem_ld_wait(a1);
-                            } else {
-                                ptx::tmem_ld_wait(a0);
-                            }
-                        } else { // no rows to sum over
-#pragma unroll
-                            for (int j = 0; j < EW::CH; ++j) a[j] = 0u;
-                        }
-                        if (k + 1u == mine) release(bar_i);
+                        TmemPieces<PIECE> pieces{tacc + (hw + EPI_SETS * k) * EW::CH, EW::CH / PIECE, c.kb1 == c.kb0};
                         if (epp->streamed && k > 0u && k - 1u + epp->bufs < mine) {
                             ew.buffers_free(); // the chunk before this one left from the buffer asked for now
                             ew.request(epp->bufs - 1u, row0, col(k - 1u + epp->bufs), c.z_out);
                         }
                         __syncwarp(); // (the biases of the chunk before have been read)
-                        ok = ew.finish(c, row0, col(k), c.end, bias_row, a);
+                        ok = ew.finish(c, row0, col(k), c.end, bias_row, pieces, [&] { if (k + 1u == mine) release(bar_i); });
                         if (!ok) break;
                         if (k + 1u < mine) ew.prefetch_bias(c, col(k + 1u));
                     }
@@ -1754,7 +1840,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             for (uint32_t ch = 0; ch < static_cast<uint32_t>(NCH); ++ch) {
                 const uint32_t owner = ch % ks;
                 if (owner == krank) continue;
-                if (EP && ((ch / ks) & 1u) != hw) continue;
+                if (EP && (ch / ks) % EPI_SETS != hw) continue;
                 // (within a warp's slot the 16-byte units are laid out [unit][lane]: every store and
                 // load instruction of the warp covers 512 contiguous bytes)
                 const uint32_t local  = ring + (((ch / ks) * ks + krank) * 4u + q) * WSLOT + lane * 16u;
@@ -1789,7 +1875,34 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             };
             [[maybe_unused]] auto ew = make_ew();
 #pragma unroll 1
-            for (uint32_t ch = krank + (EP ? hw * ks : 0u); ch < static_cast<uint32_t>(NCH); ch += (EP ? 2u : 1u) * ks) {
+            for (uint32_t ch = krank + (EP ? hw * ks : 0u); ch < static_cast<uint32_t>(NCH); ch += (EP ? EPI_SETS : 1u) * ks) {
+                if constexpr (EP) {
+                    ClusterPieces<TR ? COLUMN_PIECE : PIECE> pieces{tacc + ch * O_CH, ring + ((ch / ks) * ks * 4u + q) * WSLOT + lane * 16u, 4u * WSLOT, ks, krank};
+                    dep_wait();
+                    if constexpr (TR) {
+                        const EpilogueColumns<OUT> ec{p, *epp, lane};
+                        const uint32_t i    = ks_c.m0 + q * 32u + lane;
+                        const bool     live = (q * 32u + lane) < p.bm && i < p.M;
+                        const uint32_t col0 = ks_c.n0 + ch * 32u;
+                        const uint32_t bs   = BN < 32 ? BN : 32;
+                        const uint32_t n    = col0 < p.N ? min(min(32u, BN - ch * 32u), p.N - col0) : 0u;
+                        float          side[COLUMN_PIECE];
+                        if (epp->streamed) ec.load_side(ks_c, col0, min(n, static_cast<uint32_t>(COLUMN_PIECE)), i, live, side);
+                        ec.chunk(ks_c, col0, n, i, live, ks_c.z_out * epp->part_blocks + col0 / bs,
+                                 ks_c.z_out * epp->part_blocks + ks_c.m0 / p.bm * 4u + q, pieces, bs / COLUMN_PIECE, side, [] {});
+                    } else {
+                        const uint32_t col0 = ks_c.n0 + ch * O_CH;
+                        if (row_live && col0 < p.N) {
+                            if (epp->streamed) {
+                                ew.buffers_free();
+                                ew.request(0u, row0, col0, ks_c.z_out);
+                            }
+                            ew.prefetch_bias(ks_c, col0);
+                            __syncwarp();
+                            if (!ew.finish(ks_c, row0, col0, p.M, ew.row_bias(ks_c, row0 + lane), pieces, [] {})) break;
+                        }
+                    }
+                } else {
                 uint32_t own[O_CH];
                 float    acc[O_CH];
 #pragma unroll
@@ -1823,32 +1936,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         }
                     }
                 }
-                if constexpr (EP && TR) {
-                    const EpilogueColumns<OUT> ec{p, *epp, lane};
-                    const uint32_t i    = ks_c.m0 + q * 32u + lane;
-                    const bool     live = (q * 32u + lane) < p.bm && i < p.M;
-                    const uint32_t col0 = ks_c.n0 + ch * 32u;
-                    const uint32_t bs   = BN < 32 ? BN : 32;
-                    const uint32_t n    = col0 < p.N ? min(min(32u, BN - ch * 32u), p.N - col0) : 0u;
-                    float          side[32];
-                    dep_wait();
-                    if (epp->streamed) ec.load_side(ks_c, col0, n, i, live, side);
-                    uint32_t (&bits)[32] = reinterpret_cast<uint32_t(&)[32]>(acc);
-                    if (n) ec.finish(ks_c, col0, n, i, live, ks_c.z_out * epp->part_blocks + col0 / bs,
-                                     ks_c.z_out * epp->part_blocks + ks_c.m0 / p.bm * 4u + q, bits, side);
-                } else if constexpr (EP) {
-                    const uint32_t col0 = ks_c.n0 + ch * O_CH;
-                    if (row_live && col0 < p.N) {
-                        dep_wait();
-                        if (epp->streamed) {
-                            ew.buffers_free();
-                            ew.request(0u, row0, col0, ks_c.z_out);
-                        }
-                        ew.prefetch_bias(ks_c, col0);
-                        __syncwarp();
-                        if (!ew.finish(ks_c, row0, col0, p.M, ew.row_bias(ks_c, row0 + lane), reinterpret_cast<const uint32_t(&)[O_CH]>(acc))) break;
-                    }
-                } else if constexpr (TR) {
+                if constexpr (TR) {
                     // D(i, j) goes to out[j * M + i]: for a fixed column the warp writes 32
                     // consecutive elements (see the transposed epilogue above).
                     const uint32_t i      = ks_c.m0 + q * 32u + lane;
@@ -1894,6 +1982,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                     ++nstore;
                 }
                 } // staged store
+                } // without an epilogue
             }
             if (warp == 2 && lane == 0) B200_TL(20);
             if constexpr (EP && !TR) ew.drain();
@@ -1978,7 +2067,7 @@ __global__ void __launch_bounds__(EPI_THREADS, 1)
 // reading the next group's rows.  One warp per group.
 static __global__ void __launch_bounds__(32)
     ragged_maps_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                       CUtensorMap* __restrict__ maps, const int32_t* __restrict__ offsets, uint32_t rows)
+                       CUtensorMap* __restrict__ maps, const int32_t* offsets, uint32_t rows)
 {
     const uint32_t e = blockIdx.x, lane = threadIdx.x;
     ptx::grid_dep_launch();
