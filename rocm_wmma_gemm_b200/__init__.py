@@ -225,6 +225,9 @@ class loader:
                 return None
         else:
             handle = int(getattr(stream, "cuda_stream", stream))
+        return self._cell(handle)
+
+    def _cell(self, handle):
         cell = self._streams.get(handle)
         if cell is None:
             box = ctypes.c_void_p(handle)
@@ -266,61 +269,79 @@ class loader:
                                         int(layout_c), int(layout_a), int(layout_b)))
 
     # ---- products with epilogues, grouped products, gradients ------------------------------
-    def _place(self, stream, tensors, roles):
-        """Stream cell for a call on `tensors`, and the device to make current (None: already is).
+    def _arguments(self, stream, spec):
+        """(device to make current or None, stream cell, addresses) of a call's array arguments.
 
-        Tensors must share one CUDA device, be dense (contiguous; every shape is given by the
-        sizes of the call) and be at least as long as the call needs; raw addresses are taken as
-        they are.  The call runs on the tensors' device and, where no stream is given, on that
-        device's current stream."""
-        device = None
-        for (name, size, kind), t in zip(roles, tensors):
-            if t is None or isinstance(t, int):
-                continue
-            if not t.is_cuda or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous CUDA tensor")
-            if device is None:
-                device = t.device
-            elif t.device != device:
-                raise ValueError(f"{name} is on {t.device}, other arguments on {device}")
-            if t.numel() < size:
-                raise ValueError(f"{name} holds {t.numel()} elements, the call needs {size}")
-            if kind is not None and t.dtype != kind:
-                raise ValueError(f"{name} is {t.dtype}, not {kind}")
+        `spec` holds (name, array, elements the call needs, dtype or None).  Tensors must share one
+        CUDA device, be dense (contiguous; every shape is given by the sizes of the call) and at
+        least as long as the call needs; raw addresses are taken as they are.  The call runs on
+        the tensors' device and, where no stream is given, on that device's current stream."""
+        device, addresses = None, []
+        for name, t, size, dtype in spec:
+            if t is None:
+                addresses.append(None)
+            elif isinstance(t, int):
+                addresses.append(t)
+            else:
+                d = t.get_device()
+                if device is None:
+                    device = d
+                if d < 0 or d != device or t.numel() < size or (dtype is not None and t.dtype != dtype) or not t.is_contiguous():
+                    self._refuse(name, t, size, dtype, device)
+                addresses.append(t.data_ptr())
         if device is None:
-            return self._stream_ptr(stream), None
-        import torch
+            return None, self._stream_ptr(stream), addresses
+        if loader._raw_stream is None:
+            import torch
+            loader._torch_cuda = torch.cuda
+            loader._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+                lambda index: torch.cuda.current_stream(index).cuda_stream)
+            loader._raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         if stream is None:
-            stream = torch.cuda.current_stream(device)
-        elif getattr(stream, "device", device) != device:
-            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-        return self._stream_ptr(stream), (device if device.index != torch.cuda.current_device() else None)
+            handle = loader._raw_stream(device)
+        else:
+            owner = getattr(stream, "device_index", device)
+            if owner != device:
+                raise ValueError(f"the stream is on device {owner}, the tensors on device {device}")
+            handle = int(getattr(stream, "cuda_stream", stream))
+        return (device if loader._raw_device() != device else None), self._cell(handle), addresses
+
+    _raw_stream = _raw_device = _torch_cuda = None  # filled on the first call with tensors
+
+    @staticmethod
+    def _refuse(name, t, size, dtype, device):
+        if not t.is_cuda or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous CUDA tensor")
+        if t.get_device() != device:
+            raise ValueError(f"{name} is on {t.device}, other arguments on device {device}")
+        if t.numel() < size:
+            raise ValueError(f"{name} holds {t.numel()} elements, the call needs {size}")
+        raise ValueError(f"{name} is {t.dtype}, not {dtype}")
 
     @staticmethod
     def _on(device, call, *args) -> None:
         if device is None:
             st = call(*args)
         else:
-            import torch
-            with torch.cuda.device(device):
+            with loader._torch_cuda.device(device):
                 st = call(*args)
         if st != 0:
             _check(st)
 
     @staticmethod
-    def _epilogue(activation, gradient, bias, residual, preact, bias_grad, bias_stride):
+    def _activation(activation) -> int:
         act = ACTIVATIONS.get(activation, activation)
         if not isinstance(act, int):
             raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
-        return Epilogue(act, int(gradient), _ptr(bias), _ptr(residual), _ptr(preact), _ptr(bias_grad), bias_stride)
+        return act
 
     @staticmethod
-    def _f32(*tensors):
-        """torch.float32 if any of `tensors` is a tensor (else torch is not needed)."""
-        if all(t is None or isinstance(t, int) for t in tensors):
+    def _torch_type(t, name):
+        """torch's dtype `name` where t is a tensor (raw addresses need no torch)."""
+        if t is None or isinstance(t, int):
             return None
         import torch
-        return torch.float32
+        return getattr(torch, name)
 
     def gemm_fused(self, C, A, B, M, N, K, layout_c=0, layout_a=0, layout_b=0, batch_count=1, activation="none",
                    bias=None, residual=None, preact=None, gradient=False, bias_grad=None, bias_stride=0,
@@ -335,13 +356,14 @@ class loader:
         the sum over them), N or more gives each its own."""
         t = self._type_index(C, A, types)
         mn, vec = batch_count * M * N, N + (batch_count - 1) * bias_stride if N else 0
-        ct = getattr(C, "dtype", None)
-        sp, dev = self._place(stream, (C, A, B, bias, residual, preact, bias_grad), (
-            ("C", mn, None), ("A", batch_count * M * K, None), ("B", batch_count * K * N, getattr(A, "dtype", None)),
-            ("bias", vec, ct), ("residual", mn, ct), ("preact", mn, ct), ("bias_grad", vec, self._f32(bias_grad))))
-        epi = self._epilogue(activation, gradient, bias, residual, preact, bias_grad, bias_stride)
-        self._on(dev, self._lib.b200_gemm_fused, t, _ptr(C), _ptr(A), _ptr(B), M, N, K, batch_count, int(layout_c),
-                 int(layout_a), int(layout_b), sp, ctypes.byref(epi))
+        ct, it = getattr(C, "dtype", None), getattr(A, "dtype", None)
+        dev, sp, (c, a, b, bi, re, pr, bg) = self._arguments(stream, (
+            ("C", C, mn, None), ("A", A, batch_count * M * K, None), ("B", B, batch_count * K * N, it),
+            ("bias", bias, vec, ct), ("residual", residual, mn, ct), ("preact", preact, mn, ct),
+            ("bias_grad", bias_grad, vec, self._torch_type(bias_grad, "float32"))))
+        epi = Epilogue(self._activation(activation), int(gradient), bi, re, pr, bg, bias_stride)
+        self._on(dev, self._lib.b200_gemm_fused, t, c, a, b, M, N, K, batch_count, int(layout_c), int(layout_a),
+                 int(layout_b), sp, ctypes.byref(epi))
 
     def gemm_grouped(self, C, A, B, offsets, rows, N, K, groups, layout_b=0, activation="none", bias=None,
                      residual=None, preact=None, gradient=False, bias_grad=None, stream=None, types=None) -> None:
@@ -351,21 +373,15 @@ class loader:
         left as they are.  bias and bias_grad are groups x N.  The input gradient is the same call
         on the output's gradient with layout_b flipped and N and K exchanged."""
         t = self._type_index(C, A, types)
-        mn, ct = rows * N, getattr(C, "dtype", None)
-        sp, dev = self._place(stream, (C, A, B, bias, residual, preact, bias_grad, offsets), (
-            ("C", mn, None), ("A", rows * K, None), ("B", groups * K * N, getattr(A, "dtype", None)),
-            ("bias", groups * N, ct), ("residual", mn, ct), ("preact", mn, ct),
-            ("bias_grad", groups * N, self._f32(bias_grad)), ("offsets", groups + 1, self._int32(offsets))))
-        epi = self._epilogue(activation, gradient, bias, residual, preact, bias_grad, 0)
-        self._on(dev, self._lib.b200_gemm_grouped, t, _ptr(C), _ptr(A), _ptr(B), _ptr(offsets), rows, N, K, groups,
-                 int(layout_b), sp, ctypes.byref(epi))
-
-    @staticmethod
-    def _int32(t):
-        if t is None or isinstance(t, int):
-            return None
-        import torch
-        return torch.int32
+        mn, ct, it = rows * N, getattr(C, "dtype", None), getattr(A, "dtype", None)
+        dev, sp, (c, a, b, bi, re, pr, bg, off) = self._arguments(stream, (
+            ("C", C, mn, None), ("A", A, rows * K, None), ("B", B, groups * K * N, it),
+            ("bias", bias, groups * N, ct), ("residual", residual, mn, ct), ("preact", preact, mn, ct),
+            ("bias_grad", bias_grad, groups * N, self._torch_type(bias_grad, "float32")),
+            ("offsets", offsets, groups + 1, self._torch_type(offsets, "int32"))))
+        epi = Epilogue(self._activation(activation), int(gradient), bi, re, pr, bg, 0)
+        self._on(dev, self._lib.b200_gemm_grouped, t, c, a, b, off, rows, N, K, groups, int(layout_b), sp,
+                 ctypes.byref(epi))
 
     def gemm_grouped_wgrad(self, C, A, B, offsets, rows, M, N, groups, layout_c=0, accumulate=False, stream=None,
                            types=None) -> None:
@@ -373,11 +389,11 @@ class loader:
         C_e with `accumulate`), A rows x M, B rows x N, C groups x M x N, each C_e in layout_c.
         An empty group's C_e is zero."""
         t = self._type_index(C, A, types)
-        sp, dev = self._place(stream, (C, A, B, offsets), (
-            ("C", groups * M * N, None), ("A", rows * M, None), ("B", rows * N, getattr(A, "dtype", None)),
-            ("offsets", groups + 1, self._int32(offsets))))
-        self._on(dev, self._lib.b200_gemm_grouped_wgrad, t, _ptr(C), _ptr(A), _ptr(B), _ptr(offsets), rows, M, N,
-                 groups, int(layout_c), int(accumulate), sp)
+        dev, sp, (c, a, b, off) = self._arguments(stream, (
+            ("C", C, groups * M * N, None), ("A", A, rows * M, None), ("B", B, rows * N, getattr(A, "dtype", None)),
+            ("offsets", offsets, groups + 1, self._torch_type(offsets, "int32"))))
+        self._on(dev, self._lib.b200_gemm_grouped_wgrad, t, c, a, b, off, rows, M, N, groups, int(layout_c),
+                 int(accumulate), sp)
 
     _OUT_TYPES = None  # torch dtype of C -> a type pair with that output
 
@@ -396,14 +412,12 @@ class loader:
             t = TYPE_PAIRS[types] if isinstance(types, tuple) else int(types)
         mn, ct = batch_count * M * N, getattr(dY, "dtype", None)
         vec = groups * N if groups else (N + (batch_count - 1) * bias_stride if N else 0)
-        sp, dev = self._place(stream, (dZ, dY, preact, bias_grad, offsets), (
-            ("dZ", mn, ct), ("dY", mn, None), ("preact", mn, ct), ("bias_grad", vec, self._f32(bias_grad)),
-            ("offsets", groups + 1, self._int32(offsets))))
-        act = ACTIVATIONS.get(activation, activation)
-        if not isinstance(act, int):
-            raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
-        self._on(dev, self._lib.b200_gemm_activation_backward, t, _ptr(dZ), _ptr(dY), _ptr(preact), M, N, batch_count,
-                 int(layout), act, _ptr(bias_grad), bias_stride, _ptr(offsets), groups, sp)
+        dev, sp, (dz, dy, z, bg, off) = self._arguments(stream, (
+            ("dZ", dZ, mn, ct), ("dY", dY, mn, None), ("preact", preact, mn, ct),
+            ("bias_grad", bias_grad, vec, self._torch_type(bias_grad, "float32")),
+            ("offsets", offsets, groups + 1, self._torch_type(offsets, "int32"))))
+        self._on(dev, self._lib.b200_gemm_activation_backward, t, dz, dy, z, M, N, batch_count, int(layout),
+                 self._activation(activation), bg, bias_stride, off, groups, sp)
 
 
 def get_gemm_params(m: int, n: int, k: int, layout_c=0, layout_a=0, layout_b=0, type_group: int = 0):

@@ -1088,6 +1088,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
     __shared__ volatile uint32_t     s_abort;
     static_assert(!EP || !GATHER, "no gathering kernels with an epilogue");
     constexpr int                    EPW = EP ? EPI_WARPS : 4; // epilogue warps
+    __shared__ volatile uint32_t     s_seen[2];                                          // EP: the accumulator awaited last is complete
     __shared__ __align__(8) uint64_t s_in[EP && !TR ? EPI_WARPS * 2 : 1];                // EP: chunk of the read matrix landed
     __shared__ __align__(16) uint8_t s_bias[EP && !TR ? EPI_WARPS * 128 : 16];           // EP: a chunk's biases, per warp
 
@@ -1536,11 +1537,23 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                 else ptx::mbar_arrive(ptx::smem_u32(&s_tempty[bar_i]));
             }
         };
+        // One warp polls the accumulator's barrier, the others sleep at a named barrier: eight polling
+        // warps took issue slots and power from the producer and MMA threads (4096 x 5120 x 5120 with a
+        // residual 176 -> 164 us, the plain product 160).  Every warp calls this once per accumulator and
+        // gets the same answer (s_seen alternates: the poller is at most one accumulator ahead).
+        uint32_t waits = 0;
         auto accumulator = [&](uint32_t bar_i, uint32_t parity) -> bool {
-            bool r = bounded_wait(ptx::smem_u32(&s_tfull[bar_i]), parity, &s_abort, p.status, ST_EPI_WAIT);
-            r      = __all_sync(0xffffffffu, r);
+            const uint32_t at = waits++ & 1u;
+            if (warp == 2u) {
+                const bool r = bounded_wait(ptx::smem_u32(&s_tfull[bar_i]), parity, &s_abort, p.status, ST_EPI_WAIT);
+                const bool a = __all_sync(0xffffffffu, r);
+                if (lane == 0) s_seen[at] = a ? 1u : 0u;
+            }
+            ptx::named_barrier(1u, 32u * EPI_WARPS);
+            if (s_seen[at] == 0u) return false;
+            (void)ptx::mbar_test_wait(ptx::smem_u32(&s_tfull[bar_i]), parity); // (completed: orders this warp behind it too)
             ptx::tc_fence_after();
-            return r;
+            return true;
         };
         if constexpr (KS) {
             // one tile per cluster; the partials are summed after the cluster barriers below
@@ -1589,10 +1602,11 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             const uint32_t per_warp = (epp->bufs + epp->aux) * EPI_BUF_BYTES;
             EW ew{p, *epp, *em, tmD, p.out, lane, epi + (warp - 2u) * per_warp, ptx::smem_u32(&s_in[(warp - 2u) * 2u]),
                   &s_bias[(warp - 2u) * 128u], &s_abort};
+            bool live_warp = true;
             for (; ok && next_work(cur, c); ++it) {
                 const uint32_t buf = it % NUM_ACC;
 #pragma unroll 1
-                for (uint32_t hh = 0; hh < static_cast<uint32_t>(NSUB); ++hh) {
+                for (uint32_t hh = 0; ok && hh < static_cast<uint32_t>(NSUB); ++hh) {
                     const uint32_t bar_i  = (NSUB == 2) ? hh : buf;
                     const uint32_t parity = (NSUB == 2) ? (it & 1u) : ((it / NUM_ACC) & 1u);
                     const uint32_t colh   = c.n0 + hh * UMMA_N;
@@ -1603,7 +1617,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                     auto           col    = [&](uint32_t k) { return colh + (hw + EPI_SETS * k) * EW::CH; };
                     const uint32_t tacc   = tmem_base + ((q * 32u) << 16) + (NSUB == 2 ? hh * UMMA_N : buf * ACC_COLS);
                     float          bias_row = 0.f;
-                    if (mine) {
+                    if (mine && live_warp) {
                         dep_wait();
                         if (epp->streamed) {
                             ew.buffers_free();
@@ -1614,6 +1628,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                     }
                     ok = accumulator(bar_i, parity);
                     if (!ok) break;
+                    if (!live_warp) continue; // (it still meets the others at every accumulator)
                     if (mine == 0u) release(bar_i);
 #pragma unroll 1
                     for (uint32_t k = 0; k < mine; ++k) {
@@ -1623,11 +1638,10 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                             ew.request(epp->bufs - 1u, row0, col(k - 1u + epp->bufs), c.z_out);
                         }
                         __syncwarp(); // (the biases of the chunk before have been read)
-                        ok = ew.finish(c, row0, col(k), c.end, bias_row, pieces, [&] { if (k + 1u == mine) release(bar_i); });
-                        if (!ok) break;
+                        live_warp = ew.finish(c, row0, col(k), c.end, bias_row, pieces, [&] { if (k + 1u == mine) release(bar_i); });
+                        if (!live_warp) break; // (a wait ran out: the abort flag ends the other roles)
                         if (k + 1u < mine) ew.prefetch_bias(c, col(k + 1u));
                     }
-                    if (!ok) break;
                 }
             }
             ew.drain();

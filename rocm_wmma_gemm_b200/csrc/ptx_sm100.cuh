@@ -130,6 +130,12 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
     return ok != 0;
 }
 
+// Barrier `id` (1 .. 15) of the `threads` threads that call it (whole warps).
+__device__ __forceinline__ void named_barrier(uint32_t id, uint32_t threads)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 // ---------------------------------------------------------------- TMA
 // L2 eviction-priority policy for TMA traffic (the operand of .L2::cache_hint):
 // 0 = normal, 1 = evict first (data read or written once), 2 = evict last (panels that later
