@@ -37,7 +37,6 @@ NVCC_FLAGS = [
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",
     "-diag-suppress", "177",
-    "-split-compile", "0",  # the kernels of one file are compiled on all cores
 ]
 
 

@@ -598,7 +598,7 @@ __device__ __forceinline__ float warp_column_sums(float (&v)[N], uint32_t lane)
 // The epilogues work in pieces of 32 columns (16 where the accumulator is read transposed), in
 // loops that are not unrolled: the whole of a piece - bias, activation, residual, conversion - is a few
 // hundred instructions, which stay in the instruction cache.
-constexpr int PIECE = 32, COLUMN_PIECE = 16;
+constexpr int PIECE = 16, COLUMN_PIECE = 16;
 
 template <int N>
 __device__ __forceinline__ void tmem_ld_piece(uint32_t addr, uint32_t (&r)[N])
@@ -620,11 +620,16 @@ struct TmemPieces {
     template <class F>
     __device__ __forceinline__ void get(uint32_t i, float (&v)[N], F&& done)
     {
-        uint32_t t[N];
-        tmem_ld_piece(addr + i * N, t);
-        ptx::tmem_ld_wait(t);
+        if (empty) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = empty ? 0.f : __uint_as_float(t[j]);
+            for (int j = 0; j < N; ++j) v[j] = 0.f;
+        } else {
+            uint32_t t[N];
+            tmem_ld_piece(addr + i * N, t);
+            ptx::tmem_ld_wait(t);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = __uint_as_float(t[j]);
+        }
         if (i + 1u == count) done();
     }
 };
@@ -803,7 +808,7 @@ struct EpilogueWarp {
         for (uint32_t u = 0; u < 8; ++u) {
             if (col0 + u * UNIT < p.N) {
                 uint4 w;
-                ptx::ld_shared_v4(rowaddr + ((u ^ (lane & 7u)) << 4), w.x, w.y, w.z, w.w);
+                ptx::ld_shared_v4(rowaddr ^ (u << 4), w.x, w.y, w.z, w.w);
                 *reinterpret_cast<uint4*>(static_cast<T*>(base) + static_cast<uint64_t>(row) * p.N + col0 + u * UNIT) = w;
             }
         }
@@ -815,8 +820,10 @@ struct EpilogueWarp {
                                            Pieces& pieces, F&& accumulators_read)
     {
         const uint32_t b    = slot(0);
-        const uint32_t sbuf = stg + b * EPI_BUF_BYTES, rowaddr = sbuf + lane * 128u;
-        const uint32_t xbuf = stg + ep.bufs * EPI_BUF_BYTES, xrow = xbuf + lane * 128u;
+        const uint32_t sbuf = stg + b * EPI_BUF_BYTES, xbuf = stg + ep.bufs * EPI_BUF_BYTES;
+        // 16-byte unit u of this lane's row lies at (buffer + row_at) ^ (u << 4): the 128-byte swizzle
+        const uint32_t row_at  = lane * 128u + ((lane & 7u) << 4);
+        const uint32_t rowaddr = sbuf + row_at, xrow = xbuf + row_at;
         const uint32_t row  = row0 + lane;
         const bool     col_bias = ep.bias && !ep.bias_on_rows;
         if (col_bias) {
@@ -840,7 +847,7 @@ struct EpilogueWarp {
 #pragma unroll 1
         for (uint32_t pc = 0; pc < CH / PIECE; ++pc) {
             constexpr uint32_t UNITS = PIECE / UNIT; // 16-byte units of a row's piece
-            auto  at = [&](uint32_t i) { return ((pc * UNITS + i) ^ (lane & 7u)) << 4; }; // (128-byte swizzle)
+            const uint32_t first = (pc * UNITS) << 4, srow = rowaddr ^ first, xr = xrow ^ first;
             float v[PIECE];
             pieces.get(pc, v, accumulators_read);
             if (ep.gradient) {
@@ -849,7 +856,7 @@ struct EpilogueWarp {
 #pragma unroll
                     for (uint32_t i = 0; i < UNITS; ++i) {
                         uint32_t w[4];
-                        ptx::ld_shared_v4(rowaddr + at(i), w[0], w[1], w[2], w[3]);
+                        ptx::ld_shared_v4(srow ^ (i << 4), w[0], w[1], w[2], w[3]);
                         unpack16<OUT>(w, z + i * UNIT);
                     }
                     apply_slope(ep, v, z);
@@ -873,7 +880,7 @@ struct EpilogueWarp {
                     for (uint32_t i = 0; i < UNITS; ++i) {
                         uint32_t w[4];
                         pack16<OUT>(v + i * UNIT, w);
-                        st_shared_v4(xrow + at(i), w[0], w[1], w[2], w[3]);
+                        st_shared_v4(xr ^ (i << 4), w[0], w[1], w[2], w[3]);
                     }
                 }
                 apply_activation(ep, v);
@@ -882,7 +889,7 @@ struct EpilogueWarp {
                     for (uint32_t i = 0; i < UNITS; ++i) {
                         uint32_t w[4];
                         float    r[UNIT];
-                        ptx::ld_shared_v4(rowaddr + at(i), w[0], w[1], w[2], w[3]);
+                        ptx::ld_shared_v4(srow ^ (i << 4), w[0], w[1], w[2], w[3]);
                         unpack16<OUT>(w, r);
                         add_values(v + i * UNIT, r);
                     }
@@ -892,7 +899,7 @@ struct EpilogueWarp {
             for (uint32_t i = 0; i < UNITS; ++i) {
                 uint32_t w[4];
                 pack16<OUT>(v + i * UNIT, w);
-                st_shared_v4(rowaddr + at(i), w[0], w[1], w[2], w[3]);
+                st_shared_v4(srow ^ (i << 4), w[0], w[1], w[2], w[3]);
             }
             if (ep.part) {
                 // (what lies outside C may be NaN: a zero-filled operand times an infinity)
