@@ -48,6 +48,7 @@ struct EpilogueParams {
     uint32_t           bias_on_rows; // the bias runs along the kernel view's rows, not its columns
     uint32_t           streamed;     // a matrix is read through the staging buffers (EpilogueMaps::in)
     uint32_t           aux;          // Z is written (EpilogueMaps::aux)
+    uint32_t           plain;        // nothing but the conversion to C's type
     uint32_t           bufs;         // staging buffers per warp for C: 1 or 2
     uint32_t           table_at;     // ragged: byte offset of the group table in dynamic shared memory
     const CUtensorMap* maps;         // ragged K: two maps per group, their row extents ending at the group's end

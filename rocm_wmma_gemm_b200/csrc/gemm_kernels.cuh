@@ -814,6 +814,62 @@ struct EpilogueWarp {
         }
     }
 
+    // The staged chunk in buffer `sbuf` (and Z in `xbuf`) to memory.
+    __device__ __forceinline__ void store(const WorkCoord& c, uint32_t row0, uint32_t col0, uint32_t end, uint32_t sbuf, uint32_t xbuf)
+    {
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (ep.ragged == RAGGED_ROWS && row0 + 32u > end) {
+            // the block's last rows belong to the next group: row by row, straight from the buffer
+            const uint32_t row = row0 + lane, row_at = lane * 128u + ((lane & 7u) << 4);
+            if (row < end) {
+                store_row_from(sbuf + row_at, out, row, col0);
+                if (ep.aux) store_row_from(xbuf + row_at, ep.preact, row, col0);
+            }
+        } else if (lane == 0) {
+            ptx::tma_store_3d(&tmD, sbuf, col0, row0, c.z_out, 0);
+            if (ep.aux) ptx::tma_store_3d(&em.aux, xbuf, col0, row0, c.z_out, 0);
+        }
+        if (lane == 0) ptx::tma_store_commit(); // (an empty group keeps the count of the waits)
+        ++count;
+    }
+
+    // The same for a chunk that is only converted: no branch but the ones above.
+    template <class F>
+    __device__ __forceinline__ void finish_plain(const WorkCoord& c, uint32_t row0, uint32_t col0, uint32_t end, uint32_t acc, bool empty,
+                                                 F&& accumulators_read)
+    {
+        const uint32_t sbuf = stg + slot(0) * EPI_BUF_BYTES, row = sbuf + lane * 128u + ((lane & 7u) << 4);
+        uint32_t       t[PARTS][32];
+        if (empty) {
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) t[h][j] = 0u;
+        } else {
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) ptx::tmem_ld_32x32(acc + h * 32u, t[h]);
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) ptx::tmem_ld_wait(t[h]);
+        }
+        accumulators_read();
+        if (lane == 0) {
+            if (ep.bufs == 1u) ptx::tma_store_wait_read<0>();
+            else ptx::tma_store_wait_read<1>();
+        }
+        __syncwarp();
+#pragma unroll
+        for (uint32_t u = 0; u < 8; ++u) {
+            if constexpr (OUT == OUT_F32) {
+                st_shared_v4(row ^ (u << 4), t[0][4 * u], t[0][4 * u + 1], t[0][4 * u + 2], t[0][4 * u + 3]);
+            } else {
+                const uint32_t* v = &t[u / 4][(u % 4) * 8];
+                st_shared_v4(row ^ (u << 4), pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3]), pack2<OUT>(v[4], v[5]), pack2<OUT>(v[6], v[7]));
+            }
+        }
+        store(c, row0, col0, end, sbuf, sbuf);
+    }
+
     // The chunk at (row0, col0) from its accumulators; `end` bounds the rows.  False: a wait ran out.
     template <class Pieces, class F>
     __device__ __forceinline__ bool finish(const WorkCoord& c, uint32_t row0, uint32_t col0, uint32_t end, float bias_row,
@@ -920,20 +976,7 @@ struct EpilogueWarp {
         }
         if (ep.part && ep.bias_on_rows && row < end)
             ep.part[(static_cast<uint64_t>(c.z_out) * ep.part_blocks + col0 / CH) * p.M + row] = row_sum;
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-        if (ep.ragged == RAGGED_ROWS && row0 + 32u > end) {
-            // the block's last rows belong to the next group: row by row, straight from the buffer
-            if (row < end) {
-                store_row_from(rowaddr, out, row, col0);
-                if (ep.aux) store_row_from(xrow, ep.preact, row, col0);
-            }
-        } else if (lane == 0) {
-            ptx::tma_store_3d(&tmD, sbuf, col0, row0, c.z_out, 0);
-            if (ep.aux) ptx::tma_store_3d(&em.aux, xbuf, col0, row0, c.z_out, 0);
-        }
-        if (lane == 0) ptx::tma_store_commit(); // (an empty group keeps the count of the waits above)
-        ++count;
+        store(c, row0, col0, end, sbuf, xbuf);
         return true;
     }
 
@@ -1639,13 +1682,18 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                     if (mine == 0u) release(bar_i);
 #pragma unroll 1
                     for (uint32_t k = 0; k < mine; ++k) {
+                        auto read = [&] { if (k + 1u == mine) release(bar_i); };
+                        if (epp->plain) {
+                            ew.finish_plain(c, row0, col(k), c.end, tacc + (hw + EPI_SETS * k) * EW::CH, c.kb1 == c.kb0, read);
+                            continue;
+                        }
                         TmemPieces<PIECE> pieces{tacc + (hw + EPI_SETS * k) * EW::CH, EW::CH / PIECE, c.kb1 == c.kb0};
                         if (epp->streamed && k > 0u && k - 1u + epp->bufs < mine) {
                             ew.buffers_free(); // the chunk before this one left from the buffer asked for now
                             ew.request(epp->bufs - 1u, row0, col(k - 1u + epp->bufs), c.z_out);
                         }
                         __syncwarp(); // (the biases of the chunk before have been read)
-                        live_warp = ew.finish(c, row0, col(k), c.end, bias_row, pieces, [&] { if (k + 1u == mine) release(bar_i); });
+                        live_warp = ew.finish(c, row0, col(k), c.end, bias_row, pieces, read);
                         if (!live_warp) break; // (a wait ran out: the abort flag ends the other roles)
                         if (k + 1u < mine) ew.prefetch_bias(c, col(k + 1u));
                     }
