@@ -28,6 +28,15 @@ enum : uint32_t { RAGGED_NONE = 0, RAGGED_ROWS = 1, RAGGED_K = 2 };
 
 constexpr uint32_t MAX_GROUPS = 1024;
 
+// Division by a number the host knows, for dividends below 2^31: with l = ceil(log2 d) and
+// m = floor(2^(31 + l) / d) + 1, n / d = (n m) >> (31 + l) (m d exceeds 2^(31 + l) by at most d <= 2^l, so
+// the excess n (m d - 2^(31 + l)) / d stays below one step).  A hardware division costs an epilogue
+// warp some 150 cycles, and a tile's coordinates took four.
+struct FastDiv {
+    uint32_t d, m, shift;
+};
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv& f) { return f.d == 1u ? n : __umulhi(n, f.m) >> f.shift; }
+
 struct EpilogueParams {
     const void*    bias;        // forward: nullptr or one value per column of the caller's C, C's type
     const void*    residual;    // forward: nullptr or a matrix like C (may be C itself)
@@ -51,6 +60,7 @@ struct EpilogueParams {
     uint32_t           plain;        // nothing but the conversion to C's type
     uint32_t           bufs;         // staging buffers per warp for C: 1 or 2
     uint32_t           table_at;     // ragged: byte offset of the group table in dynamic shared memory
+    FastDiv            per_item, per_band, per_column; // tiles per batch item (ragged rows: of the other extent), per raster band, rows per band or column
     const CUtensorMap* maps;         // ragged K: two maps per group, their row extents ending at the group's end
 };
 

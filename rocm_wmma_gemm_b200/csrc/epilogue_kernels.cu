@@ -5,10 +5,10 @@ namespace b200 {
 
 namespace {
 
-template <class K>
+template <int OUT, class K>
 cudaError_t allow_smem(K kernel)
 {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)EPI_SMEM_LIMIT);
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)epilogue_smem_limit(OUT));
 }
 
 template <int BN, int CL, bool TR, bool KS>
@@ -16,13 +16,13 @@ cudaError_t set_one()
 {
     cudaError_t e;
     if constexpr (KS) {
-        e = allow_smem(gemm_epilogue_ksplit_kernel<BN, OUT_F32, TR>);
-        if (e == cudaSuccess) e = allow_smem(gemm_epilogue_ksplit_kernel<BN, OUT_F16, TR>);
-        if (e == cudaSuccess) e = allow_smem(gemm_epilogue_ksplit_kernel<BN, OUT_BF16, TR>);
+        e = allow_smem<OUT_F32>(gemm_epilogue_ksplit_kernel<BN, OUT_F32, TR>);
+        if (e == cudaSuccess) e = allow_smem<OUT_F16>(gemm_epilogue_ksplit_kernel<BN, OUT_F16, TR>);
+        if (e == cudaSuccess) e = allow_smem<OUT_BF16>(gemm_epilogue_ksplit_kernel<BN, OUT_BF16, TR>);
     } else {
-        e = allow_smem(gemm_epilogue_kernel<BN, OUT_F32, CL, TR>);
-        if (e == cudaSuccess) e = allow_smem(gemm_epilogue_kernel<BN, OUT_F16, CL, TR>);
-        if (e == cudaSuccess) e = allow_smem(gemm_epilogue_kernel<BN, OUT_BF16, CL, TR>);
+        e = allow_smem<OUT_F32>(gemm_epilogue_kernel<BN, OUT_F32, CL, TR>);
+        if (e == cudaSuccess) e = allow_smem<OUT_F16>(gemm_epilogue_kernel<BN, OUT_F16, CL, TR>);
+        if (e == cudaSuccess) e = allow_smem<OUT_BF16>(gemm_epilogue_kernel<BN, OUT_BF16, CL, TR>);
     }
     return e;
 }

@@ -133,8 +133,8 @@ constexpr uint32_t A_TILE_BYTES   = BLOCK_M * BLOCK_K * 2;
 constexpr uint32_t EPI_BUF_BYTES  = 32 * 128; // one warp's 32 rows x 128 B
 constexpr uint32_t EPI_BYTES      = 4 * 2 * EPI_BUF_BYTES;
 // Dynamic shared memory a kernel with an epilogue may use: 227 KiB minus its static part (barriers
-// and biases, under 1.5 KiB).
-constexpr uint32_t EPI_SMEM_LIMIT = 232448u - 1536u;
+// and two tiles' biases).
+__host__ __device__ constexpr uint32_t epilogue_smem_limit(int out) { return 232448u - (out == OUT_F32 ? 2560u : 1536u); }
 constexpr uint64_t WAIT_LIMIT_NS  = 2000000000ull; // 2 s per bounded wait
 
 // Bytes of one ring slot in one CTA: A' 128 x 64 plus B' (bn / cluster) x 64.
@@ -417,42 +417,70 @@ __device__ __forceinline__ void build_group_table(const EpilogueParams& ep, uint
     }
 }
 
+// tile_coords with the divisors the host has prepared.
+__device__ __forceinline__ void tile_coords_epilogue(const GemmParams& p, const EpilogueParams& ep, uint32_t t, uint32_t& m_idx, uint32_t& n_idx)
+{
+    if (p.group_m == 0u) {
+        n_idx = fast_div(t, ep.per_column);
+        m_idx = t - n_idx * p.m_tiles;
+        if (p.snake && (n_idx & 1u)) m_idx = p.m_tiles - 1u - m_idx;
+        return;
+    }
+    const uint32_t g       = fast_div(t, ep.per_band);
+    const uint32_t first_m = g * p.group_m;
+    const uint32_t gsize   = min(p.group_m, p.m_tiles - first_m);
+    const uint32_t in_g    = t - g * p.group_m * p.n_tiles;
+    n_idx                  = gsize == ep.per_column.d ? fast_div(in_g, ep.per_column) : in_g / gsize; // (the last band may be lower)
+    uint32_t m_in          = in_g - n_idx * gsize;
+    if (p.snake) {
+        if (n_idx & 1u) m_in = gsize - 1u - m_in;
+        if (g & 1u) n_idx = p.n_tiles - 1u - n_idx;
+    }
+    m_idx = first_m + m_in;
+}
+
 template <bool TR>
 __device__ __forceinline__ bool work_next_epilogue(const GemmParams& p, const EpilogueParams& ep, const GroupTable& gt,
-                                                   WorkCursor& cur, uint32_t unit, uint32_t units, int bn, int bm,
-                                                   WorkCoord& c)
+                                                   WorkCursor& cur, uint32_t units, int bn, int bm, WorkCoord& c)
 {
-    if (ep.ragged == RAGGED_NONE) {
-        if (!work_next(p, cur, unit, units, bn, bm, c)) return false;
-        c.z_a = c.z_b = c.z_in;
-        c.k_first = c.group = c.first = 0u;
-        c.end     = TR ? p.N : p.M;
-        return true;
-    }
-    if (ep.ragged == RAGGED_K) {
-        if (!work_next(p, cur, unit, units, bn, bm, c)) return false;
-        c.group = c.z_in; // (the batch index)
-        c.first = c.k_first = gt.first[c.group];
-        c.z_a = c.z_b = 0u;
-        c.end = p.M;
-        c.kb0 = 0u;
-        c.kb1 = (gt.first[c.group + 1u] - c.first + BLOCK_K - 1u) / BLOCK_K;
-        return true;
-    }
-    const uint32_t other = TR ? p.m_tiles : p.n_tiles; // tiles of the other extent
-    const uint32_t w     = cur.next;
-    if (w >= gt.tiles[ep.groups] * other) return false;
+    const uint32_t w = cur.next;
     cur.next += units;
-    uint32_t       lo = 0u, hi = ep.groups; // the group whose tiles [tiles[e], tiles[e + 1]) x other hold w
-    const uint32_t wt = w / other;
+    c.partial = 0u;
+    if (ep.ragged != RAGGED_ROWS) { // dense (the K partitions of a tile are one cluster's CTAs), or ragged K
+        if (w >= p.num_work) return false;
+        const uint32_t b = fast_div(w, ep.per_item);
+        uint32_t       m_idx, n_idx;
+        tile_coords_epilogue(p, ep, w - b * ep.per_item.d, m_idx, n_idx);
+        c.m0   = m_idx * static_cast<uint32_t>(bm);
+        c.n0   = n_idx * static_cast<uint32_t>(bn);
+        c.z_in = c.z_out = b;
+        c.end  = TR ? p.N : p.M;
+        if (ep.ragged == RAGGED_K) {
+            c.group = b;
+            c.first = c.k_first = gt.first[b];
+            c.z_a = c.z_b = c.kb0 = 0u;
+            c.kb1 = (gt.first[b + 1u] - c.first + BLOCK_K - 1u) / BLOCK_K;
+        } else {
+            c.z_a = c.z_b = b;
+            c.k_first = c.group = c.first = 0u;
+            c.kb0 = cur.krank * p.kb_per_split;
+            c.kb1 = min(p.k_blocks, c.kb0 + p.kb_per_split);
+        }
+        return true;
+    }
+    const uint32_t other = ep.per_item.d; // tiles of the other extent
+    const uint32_t wt    = fast_div(w, ep.per_item);
+    if (wt >= gt.tiles[ep.groups]) return false;
+    uint32_t lo = 0u, hi = ep.groups; // the group whose tiles [tiles[e], tiles[e + 1]) hold wt
     while (hi - lo > 1u) {
         const uint32_t mid = (lo + hi) / 2u;
         if (gt.tiles[mid] <= wt) lo = mid;
         else hi = mid;
     }
-    const uint32_t in_g  = w - gt.tiles[lo] * other;
-    const uint32_t rt    = gt.tiles[lo + 1u] - gt.tiles[lo];
-    const uint32_t o     = in_g / rt;
+    const uint32_t t0    = gt.tiles[lo];
+    const uint32_t in_g  = w - t0 * other;
+    const uint32_t rt    = gt.tiles[lo + 1u] - t0;
+    const uint32_t o     = rt == 1u ? in_g : in_g / rt;
     c.group              = lo;
     c.first              = gt.first[lo];
     c.end                = gt.first[lo + 1u];
@@ -461,10 +489,8 @@ __device__ __forceinline__ bool work_next_epilogue(const GemmParams& p, const Ep
     c.n0                 = TR ? along : o * static_cast<uint32_t>(bn);
     c.z_a                = TR ? lo : 0u;
     c.z_b                = TR ? 0u : lo;
-    c.z_in = c.z_out = 0u;
-    c.k_first = c.partial = 0u;
-    c.kb0                 = 0u;
-    c.kb1                 = p.k_blocks;
+    c.z_in = c.z_out = c.k_first = c.kb0 = 0u;
+    c.kb1            = p.k_blocks;
     return true;
 }
 
@@ -756,12 +782,11 @@ struct EpilogueWarp {
     uint32_t                 lane;
     uint32_t                 stg;     // staging buffers: ep.bufs for C, then one for Z
     uint32_t                 in_bar;  // barriers of the first two
-    uint8_t*                 bias_sm; // CH biases in C's type (128 bytes)
+    uint8_t*                 bias_sm; // the tile's biases, in C's type
     volatile uint32_t*       s_abort;
     uint32_t                 count     = 0; // chunks so far: the next one's buffer is count % ep.bufs
     uint32_t                 in_phase  = 0; // parity per buffer
     uint32_t                 in_flight = 0; // requested, not yet awaited
-    T                        bias_reg[PARTS]; // this lane's biases of the next chunk
 
     __device__ __forceinline__ uint32_t slot(uint32_t k) const { return (count + k) & (ep.bufs - 1u); }
 
@@ -785,15 +810,14 @@ struct EpilogueWarp {
         __syncwarp();
     }
 
-    __device__ __forceinline__ void prefetch_bias(const WorkCoord& c, uint32_t col0)
+    // Columns [32 w, 32 w + 32) of the tile's (tile half's) biases by epilogue warp w; the barrier before
+    // the accumulator orders them before their use.
+    __device__ __forceinline__ void fetch_bias(const WorkCoord& c, uint32_t col0, uint32_t at, uint8_t* to)
     {
+        bias_sm = to;
         if (!ep.bias || ep.bias_on_rows) return;
         const T* b = static_cast<const T*>(ep.bias) + (ep.ragged == RAGGED_ROWS ? c.group : c.z_in) * ep.bias_stride;
-#pragma unroll
-        for (int h = 0; h < PARTS; ++h) {
-            const uint32_t col = col0 + h * 32u + lane;
-            bias_reg[h]        = col < p.N ? b[col] : from_f32<T>(0.f);
-        }
+        reinterpret_cast<T*>(to)[at + lane] = col0 + at + lane < p.N ? b[col0 + at + lane] : from_f32<T>(0.f);
     }
 
     __device__ __forceinline__ float row_bias(const WorkCoord& c, uint32_t row) const
@@ -870,9 +894,10 @@ struct EpilogueWarp {
         store(c, row0, col0, end, sbuf, sbuf);
     }
 
-    // The chunk at (row0, col0) from its accumulators; `end` bounds the rows.  False: a wait ran out.
+    // The chunk at (row0, col0), column tile_col of its tile, from its accumulators; `end` bounds the
+    // rows.  False: a wait ran out.
     template <class Pieces, class F>
-    __device__ __forceinline__ bool finish(const WorkCoord& c, uint32_t row0, uint32_t col0, uint32_t end, float bias_row,
+    __device__ __forceinline__ bool finish(const WorkCoord& c, uint32_t row0, uint32_t col0, uint32_t tile_col, uint32_t end, float bias_row,
                                            Pieces& pieces, F&& accumulators_read)
     {
         const uint32_t b    = slot(0);
@@ -882,10 +907,7 @@ struct EpilogueWarp {
         const uint32_t rowaddr = sbuf + row_at, xrow = xbuf + row_at;
         const uint32_t row  = row0 + lane;
         const bool     col_bias = ep.bias && !ep.bias_on_rows;
-        if (col_bias) {
-#pragma unroll
-            for (int h = 0; h < PARTS; ++h) reinterpret_cast<T*>(bias_sm)[h * 32 + lane] = bias_reg[h];
-        }
+        const uint32_t bias_at  = ptx::smem_u32(bias_sm) + tile_col * static_cast<uint32_t>(sizeof(T));
         if (ep.streamed) {
             bool ok = bounded_wait(in_bar + 8u * b, (in_phase >> b) & 1u, s_abort, p.status, ST_EPI_WAIT);
             ok      = __all_sync(0xffffffffu, ok);
@@ -923,7 +945,7 @@ struct EpilogueWarp {
                     for (uint32_t i = 0; i < UNITS; ++i) {
                         uint32_t w[4];
                         float    t[UNIT];
-                        ptx::ld_shared_v4(ptx::smem_u32(bias_sm) + (pc * UNITS + i) * 16u, w[0], w[1], w[2], w[3]);
+                        ptx::ld_shared_v4(bias_at + (pc * UNITS + i) * 16u, w[0], w[1], w[2], w[3]);
                         unpack16<OUT>(w, t);
                         add_values(v + i * UNIT, t);
                     }
@@ -1140,7 +1162,8 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
     constexpr int                    EPW = EP ? EPI_WARPS : 4; // epilogue warps
     __shared__ volatile uint32_t     s_seen[2];                                          // EP: the accumulator awaited last is complete
     __shared__ __align__(8) uint64_t s_in[EP && !TR ? EPI_WARPS * 2 : 1];                // EP: chunk of the read matrix landed
-    __shared__ __align__(16) uint8_t s_bias[EP && !TR ? EPI_WARPS * 128 : 16];           // EP: a chunk's biases, per warp
+    constexpr uint32_t               BIAS_BYTES = (UMMA_N < 32 * EPI_WARPS ? 32 * EPI_WARPS : UMMA_N) * OUT_BYTES;
+    __shared__ __align__(16) uint8_t s_bias[EP && !TR ? 2 * BIAS_BYTES : 16];            // EP: a tile's biases, two tiles in turn
 
     const uint32_t tid    = threadIdx.x;
     const uint32_t warp   = tid >> 5;
@@ -1190,7 +1213,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
         }
     }
     auto next_work = [&](WorkCursor& cur, WorkCoord& c) -> bool {
-        if constexpr (EP) return work_next_epilogue<TR>(p, *epp, gt, cur, unit, units, wn, tile_m, c);
+        if constexpr (EP) return work_next_epilogue<TR>(p, *epp, gt, cur, units, wn, tile_m, c);
         else return work_next(p, cur, unit, units, wn, tile_m, c);
     };
 
@@ -1583,7 +1606,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             ptx::tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (CL == 2) ptx::mbar_arrive_cluster(ptx::smem_u32(&s_tempty[bar_i]), 0);
+                if constexpr (CL == 2) ptx::mbar_arrive_cluster_relaxed(ptx::smem_u32(&s_tempty[bar_i]), 0);
                 else ptx::mbar_arrive(ptx::smem_u32(&s_tempty[bar_i]));
             }
         };
@@ -1608,6 +1631,13 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
         if constexpr (KS) {
             // one tile per cluster; the partials are summed after the cluster barriers below
             if (next_work(cur, c)) {
+                if constexpr (!TR) { // the tile's biases, for the sums after the cluster barriers
+                    if (epp->bias && !epp->bias_on_rows && (warp - 2u) * 32u < static_cast<uint32_t>(BN)) {
+                        dep_wait();
+                        EpilogueWarp<OUT> ew{p, *epp, *em, tmD, p.out, lane, 0u, 0u, s_bias, &s_abort};
+                        ew.fetch_bias(c, c.n0, (warp - 2u) * 32u, s_bias);
+                    }
+                }
                 ok    = accumulator(0u, 0u);
                 ks_c  = c;
                 ks_ok = ok;
@@ -1651,7 +1681,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             using EW = EpilogueWarp<OUT>;
             const uint32_t per_warp = (epp->bufs + epp->aux) * EPI_BUF_BYTES;
             EW ew{p, *epp, *em, tmD, p.out, lane, epi + (warp - 2u) * per_warp, ptx::smem_u32(&s_in[(warp - 2u) * 2u]),
-                  &s_bias[(warp - 2u) * 128u], &s_abort};
+                  s_bias, &s_abort};
             bool live_warp = true;
             for (; ok && next_work(cur, c); ++it) {
                 const uint32_t buf = it % NUM_ACC;
@@ -1673,9 +1703,10 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                             ew.buffers_free();
                             for (uint32_t k = 0; k < min(epp->bufs, mine); ++k) ew.request(k, row0, col(k), c.z_out);
                         }
-                        ew.prefetch_bias(c, col(0));
                         bias_row = ew.row_bias(c, row0 + lane);
                     }
+                    if (epp->bias && !epp->bias_on_rows) dep_wait(); // (every warp brings its share, with or without rows of its own)
+                    ew.fetch_bias(c, colh, (warp - 2u) * 32u, s_bias + (waits & 1u) * BIAS_BYTES);
                     ok = accumulator(bar_i, parity);
                     if (!ok) break;
                     if (!live_warp) continue; // (it still meets the others at every accumulator)
@@ -1692,10 +1723,8 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                             ew.buffers_free(); // the chunk before this one left from the buffer asked for now
                             ew.request(epp->bufs - 1u, row0, col(k - 1u + epp->bufs), c.z_out);
                         }
-                        __syncwarp(); // (the biases of the chunk before have been read)
-                        live_warp = ew.finish(c, row0, col(k), c.end, bias_row, pieces, read);
+                        live_warp = ew.finish(c, row0, col(k), col(k) - colh, c.end, bias_row, pieces, read);
                         if (!live_warp) break; // (a wait ran out: the abort flag ends the other roles)
-                        if (k + 1u < mine) ew.prefetch_bias(c, col(k + 1u));
                     }
                 }
             }
@@ -1939,7 +1968,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             auto make_ew = [&]() {
                 if constexpr (EP && !TR)
                     return EpilogueWarp<OUT>{p, *epp, *em, tmD, p.out, lane, epi + (warp - 2u) * per_warp,
-                                             ptx::smem_u32(&s_in[(warp - 2u) * 2u]), &s_bias[(warp - 2u) * 128u], &s_abort};
+                                             ptx::smem_u32(&s_in[(warp - 2u) * 2u]), s_bias, &s_abort};
                 else return 0;
             };
             [[maybe_unused]] auto ew = make_ew();
@@ -1966,9 +1995,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                                 ew.buffers_free();
                                 ew.request(0u, row0, col0, ks_c.z_out);
                             }
-                            ew.prefetch_bias(ks_c, col0);
-                            __syncwarp();
-                            if (!ew.finish(ks_c, row0, col0, p.M, ew.row_bias(ks_c, row0 + lane), pieces, [] {})) break;
+                            if (!ew.finish(ks_c, row0, col0, ch * O_CH, p.M, ew.row_bias(ks_c, row0 + lane), pieces, [] {})) break;
                         }
                     }
                 } else {
