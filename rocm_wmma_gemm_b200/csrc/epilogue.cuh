@@ -1,7 +1,6 @@
 // Device side of the products with epilogues and of the grouped products: the activation
 // functions and their derivatives, the epilogue's parameters, ragged-row bookkeeping, and the
-// kernels around the tcgen05 GEMM (CUDA-core product for operands TMA cannot address, bias
-// gradient sums, backward of an activation).
+// kernels around the tcgen05 GEMM (bias gradient sums, backward of an activation).
 //
 //   forward    Z = A*B + bias      C = act(Z) + residual          (Z kept on request)
 //   gradient   C = (A*B) .* act'(Z)      bias_grad = sum of C over the rows, before rounding
@@ -53,10 +52,11 @@ struct EpilogueParams {
     const int32_t* offsets;     // ragged: groups + 1 row offsets on the device
     uint32_t       groups;
     uint32_t       rows;        // ragged: rows of the ragged operands
-    // tcgen05 kernels only
+    // the products only
     uint32_t           bias_on_rows; // the bias runs along the kernel view's rows, not its columns
     uint32_t           streamed;     // a matrix is read through the staging buffers (EpilogueMaps::in)
     uint32_t           aux;          // Z is written (EpilogueMaps::aux)
+    uint32_t           unaligned;    // TMA cannot address C or the matrices like it
     uint32_t           plain;        // nothing but the conversion to C's type
     uint32_t           bufs;         // staging buffers per warp for C: 1 or 2
     uint32_t           table_at;     // ragged: byte offset of the group table in dynamic shared memory
@@ -260,140 +260,6 @@ __device__ __forceinline__ void group_rows(const int32_t* offsets, uint32_t e, u
     for (int d = 16; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
     lo = top;
     hi = max(lo, clamp_offset(offsets[e + 1u], rows));
-}
-
-// ---------------------------------------------------------------------------------------------
-// CUDA-core product with epilogue, arbitrary element strides, f32 accumulation in ascending k:
-// a 64 x 64 tile of C per block, 4 x 4 elements per thread.  Serves what TMA cannot address
-// (a contiguous extent that is not a multiple of 16 bytes).  One kernel for the dense, the
-// grouped (ragged rows) and the weight-gradient (ragged K) products.
-// ---------------------------------------------------------------------------------------------
-struct SimpleParams {
-    const void* A;
-    const void* B;
-    void*       C;
-    uint32_t    M, N, K;
-    uint32_t    n_tiles;
-    uint64_t    a_sm, a_sk, b_sk, b_sn, c_sm, c_sn; // element strides
-    uint64_t    a_sb, b_sb, c_sb;                   // per batch item / group
-    uint32_t    z0;                                 // first batch item of this launch
-};
-
-constexpr uint32_t SIMPLE_TILE = 64;
-
-template <class TIn, class TOut>
-__global__ void __launch_bounds__(256) simple_product_kernel(const SimpleParams p, const EpilogueParams ep)
-{
-    __shared__ float    sA[16][SIMPLE_TILE + 4];
-    __shared__ float    sB[16][SIMPLE_TILE + 4];
-    __shared__ uint32_t s_where[4];
-    const uint32_t tid = threadIdx.x, tx = tid & 15u, ty = tid >> 4;
-    const uint32_t j0  = (blockIdx.x % p.n_tiles) * SIMPLE_TILE;
-    const uint32_t mt  = blockIdx.x / p.n_tiles;
-    uint32_t       z = blockIdx.z + p.z0, m0 = mt * SIMPLE_TILE, m1 = min(p.M, m0 + SIMPLE_TILE), k0 = 0u, k1 = p.K, first = 0u;
-    if (ep.ragged == RAGGED_ROWS) {
-        if (tid < 32u) {
-            uint32_t   e = 0, f = 0, r0 = 0, r1 = 0;
-            const bool ok = locate_row_tile(ep.offsets, ep.groups, ep.rows, SIMPLE_TILE, mt, e, f, r0, r1);
-            if (tid == 0) {
-                s_where[0] = ok ? e : 0xffffffffu;
-                s_where[1] = r0;
-                s_where[2] = r1;
-                s_where[3] = f;
-            }
-        }
-        __syncthreads();
-        z = s_where[0];
-        if (z == 0xffffffffu) return; // (the whole block)
-        m0    = s_where[1];
-        m1    = s_where[2];
-        first = s_where[3];
-    } else if (ep.ragged == RAGGED_K) {
-        if (tid < 32u) {
-            uint32_t lo, hi;
-            group_rows(ep.offsets, z, ep.rows, lo, hi);
-            if (tid == 0) {
-                s_where[0] = lo;
-                s_where[1] = hi;
-            }
-        }
-        __syncthreads();
-        k0 = s_where[0];
-        k1 = s_where[1];
-    }
-    // ragged rows: A and C are addressed by global row; ragged K: A and B by global row of the sum
-    const TIn* A = static_cast<const TIn*>(p.A) + (ep.ragged == RAGGED_NONE ? z * p.a_sb : 0u);
-    const TIn* B = static_cast<const TIn*>(p.B) + (ep.ragged != RAGGED_K ? z * p.b_sb : 0u);
-    const uint64_t c_base = ep.ragged != RAGGED_ROWS ? z * p.c_sb : 0u;
-
-    float acc[4][4] = {};
-    for (uint32_t k = k0; k < k1; k += 16u) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            // neighbouring threads read along whichever index is contiguous
-            const uint32_t ka = p.a_sk == 1 ? tx : ty, ma = (p.a_sk == 1 ? ty : tx) + 16u * i;
-            sA[ka][ma] = (k + ka < k1 && m0 + ma < m1) ? to_f32(A[(m0 + ma) * p.a_sm + (k + ka) * p.a_sk]) : 0.f;
-            const uint32_t kb = p.b_sk == 1 ? tx : ty, nb = (p.b_sk == 1 ? ty : tx) + 16u * i;
-            sB[kb][nb] = (k + kb < k1 && j0 + nb < p.N) ? to_f32(B[(k + kb) * p.b_sk + (j0 + nb) * p.b_sn]) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int kk = 0; kk < 16; ++kk) {
-            float a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = sA[kk][ty + 16 * i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = sB[kk][tx + 16 * j];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-        }
-        __syncthreads();
-    }
-    TOut*       C    = static_cast<TOut*>(p.C) + c_base;
-    const TOut* bias = static_cast<const TOut*>(ep.bias);
-    const TOut* res  = ep.residual ? static_cast<const TOut*>(ep.residual) + c_base : nullptr;
-    TOut*       pre  = ep.preact ? static_cast<TOut*>(ep.preact) + c_base : nullptr;
-    with_act(ep.act, [&](auto tag) {
-        constexpr uint32_t ACT = decltype(tag)::value;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t m = m0 + ty + 16u * i, n = j0 + tx + 16u * j;
-                if (m < m1 && n < p.N) {
-                    const uint64_t at = m * p.c_sm + n * p.c_sn;
-                    float          v  = acc[i][j];
-                    if (ep.gradient) {
-                        if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(pre[at]), ep));
-                    } else {
-                        if (bias) v += to_f32(bias[z * ep.bias_stride + n]);
-                        if (pre) pre[at] = from_f32<TOut>(v);
-                        v = act_value<ACT>(v, ep);
-                        if (res) v += to_f32(res[at]);
-                    }
-                    C[at]     = from_f32<TOut>(v);
-                    acc[i][j] = v;
-                } else {
-                    acc[i][j] = 0.f;
-                }
-            }
-        }
-    });
-    if (ep.part) { // column sums of the tile, rows in a fixed order
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sA[ty][tx + 16 * j] = (acc[0][j] + acc[1][j]) + (acc[2][j] + acc[3][j]);
-        __syncthreads();
-        if (tid < SIMPLE_TILE && j0 + tid < p.N) {
-            float s = 0.f;
-            for (int i = 0; i < 16; ++i) s += sA[i][tid];
-            const uint64_t block = ep.ragged == RAGGED_ROWS
-                                       ? group_first_block(first, z, SIMPLE_TILE) + (m0 - first) / SIMPLE_TILE
-                                       : static_cast<uint64_t>(z) * ep.part_blocks + mt;
-            ep.part[block * p.N + j0 + tid] = s;
-        }
-    }
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -1,6 +1,8 @@
 // The tcgen05 kernels with an epilogue: instantiations and launches.
 #include "epilogue_kernels.cuh"
 
+#include <algorithm>
+
 namespace b200 {
 
 namespace {
@@ -127,6 +129,14 @@ cudaError_t epilogue_pairs(int bn, uint32_t smem, int* pairs)
     q.numAttrs            = 1;
     return bn == 512 ? cudaOccupancyMaxActiveClusters(pairs, gemm_epilogue_kernel<512, OUT_F32, 2>, &q)
                      : cudaOccupancyMaxActiveClusters(pairs, gemm_epilogue_kernel<256, OUT_F32, 2>, &q);
+}
+
+cudaError_t launch_pad_lines(const void* src, void* dst, uint64_t lines, uint32_t length, uint32_t pitch, const FastDiv& per_line, int sm_count, cudaStream_t s)
+{
+    const uint64_t units  = lines * (pitch / 8);
+    const unsigned blocks = (unsigned)std::min<uint64_t>((units + 255) / 256, (uint64_t)sm_count * 16);
+    pad_lines_kernel<<<blocks, 256, 0, s>>>(static_cast<const uint16_t*>(src), static_cast<uint4*>(dst), units, length, per_line);
+    return cudaGetLastError();
 }
 
 cudaError_t launch_ragged_maps(const CUtensorMap& a, const CUtensorMap& b, CUtensorMap* maps, const int32_t* offsets, uint32_t groups,

@@ -766,6 +766,28 @@ __device__ __forceinline__ void pack16(const float* v, uint32_t (&w)[4])
 // load through the read-only path counts as safe to execute early: with no bias, the compiler moved
 // `__ldg(bias + i)` out of a loop and above the test of the pointer.)
 
+template <class T>
+__device__ __forceinline__ T ld_shared_elem(uint32_t addr)
+{
+    if constexpr (sizeof(T) == 4) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+        return v;
+    } else {
+        uint16_t v;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+        T t;
+        *reinterpret_cast<uint16_t*>(&t) = v;
+        return t;
+    }
+}
+template <class T>
+__device__ __forceinline__ void st_shared_elem(uint32_t addr, T t)
+{
+    if constexpr (sizeof(T) == 4) asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(t) : "memory");
+    else asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(*reinterpret_cast<const uint16_t*>(&t)) : "memory");
+}
+
 // One epilogue warp of a staged kernel with an epilogue: 32 rows x 128-byte column chunks.
 template <int OUT>
 struct EpilogueWarp {
@@ -778,7 +800,7 @@ struct EpilogueWarp {
     const EpilogueParams&    ep;
     const EpilogueMaps&      em;
     const CUtensorMap&       tmD;
-    void*                    out;     // C, for rows that may not be stored 32 at a time
+    void*                    out;     // C, for what TMA may not store
     uint32_t                 lane;
     uint32_t                 stg;     // staging buffers: ep.bufs for C, then one for Z
     uint32_t                 in_bar;  // barriers of the first two
@@ -794,6 +816,7 @@ struct EpilogueWarp {
     // stores before (request() is called after a wait on them).
     __device__ __forceinline__ void request(uint32_t k, uint32_t row0, uint32_t col0, uint32_t z)
     {
+        if (ep.unaligned) return; // (read in finish)
         const uint32_t b = slot(k);
         if (lane == 0) {
             ptx::mbar_expect_tx(in_bar + 8u * b, EPI_BUF_BYTES);
@@ -826,14 +849,24 @@ struct EpilogueWarp {
         return to_f32(static_cast<const T*>(ep.bias)[c.z_in * ep.bias_stride + row]);
     }
 
-    __device__ __forceinline__ void store_row_from(uint32_t rowaddr, void* base, uint32_t row, uint32_t col0) const
+    // Rows [row0, end) of a chunk between a staging buffer and a matrix that TMA cannot address, or a
+    // block whose last rows belong to the next group: element by element, a row's 32 or 64 elements
+    // at a time.
+    template <bool LOAD>
+    __device__ __forceinline__ void move_rows(uint32_t buf, void* base, uint32_t z, uint32_t row0, uint32_t col0, uint32_t end) const
     {
+        const uint32_t rows = min(32u, end - row0);
+        T*             at   = static_cast<T*>(base) + (static_cast<uint64_t>(z) * p.M + row0) * p.N + col0 + lane;
+#pragma unroll 4
+        for (uint32_t r = 0; r < rows; ++r, at += p.N) {
 #pragma unroll
-        for (uint32_t u = 0; u < 8; ++u) {
-            if (col0 + u * UNIT < p.N) {
-                uint4 w;
-                ptx::ld_shared_v4(rowaddr ^ (u << 4), w.x, w.y, w.z, w.w);
-                *reinterpret_cast<uint4*>(static_cast<T*>(base) + static_cast<uint64_t>(row) * p.N + col0 + u * UNIT) = w;
+            for (uint32_t h = 0; h < static_cast<uint32_t>(PARTS); ++h) {
+                const uint32_t col  = h * 32u + lane;
+                const uint32_t addr = buf + r * 128u + (((col / UNIT) ^ (r & 7u)) << 4) + (col % UNIT) * static_cast<uint32_t>(sizeof(T));
+                if (col0 + col < p.N) {
+                    if constexpr (LOAD) st_shared_elem(addr, at[h * 32u]);
+                    else at[h * 32u] = ld_shared_elem<T>(addr);
+                }
             }
         }
     }
@@ -843,13 +876,9 @@ struct EpilogueWarp {
     {
         ptx::fence_proxy_async_smem();
         __syncwarp();
-        if (ep.ragged == RAGGED_ROWS && row0 + 32u > end) {
-            // the block's last rows belong to the next group: row by row, straight from the buffer
-            const uint32_t row = row0 + lane, row_at = lane * 128u + ((lane & 7u) << 4);
-            if (row < end) {
-                store_row_from(sbuf + row_at, out, row, col0);
-                if (ep.aux) store_row_from(xbuf + row_at, ep.preact, row, col0);
-            }
+        if (ep.unaligned || (ep.ragged == RAGGED_ROWS && row0 + 32u > end)) {
+            move_rows<false>(sbuf, out, c.z_out, row0, col0, end);
+            if (ep.aux) move_rows<false>(xbuf, ep.preact, c.z_out, row0, col0, end);
         } else if (lane == 0) {
             ptx::tma_store_3d(&tmD, sbuf, col0, row0, c.z_out, 0);
             if (ep.aux) ptx::tma_store_3d(&em.aux, xbuf, col0, row0, c.z_out, 0);
@@ -908,7 +937,10 @@ struct EpilogueWarp {
         const uint32_t row  = row0 + lane;
         const bool     col_bias = ep.bias && !ep.bias_on_rows;
         const uint32_t bias_at  = ptx::smem_u32(bias_sm) + tile_col * static_cast<uint32_t>(sizeof(T));
-        if (ep.streamed) {
+        if (ep.streamed && ep.unaligned) {
+            __syncwarp();
+            move_rows<true>(sbuf, ep.gradient ? ep.preact : const_cast<void*>(ep.residual), c.z_out, row0, col0, end);
+        } else if (ep.streamed) {
             bool ok = bounded_wait(in_bar + 8u * b, (in_phase >> b) & 1u, s_abort, p.status, ST_EPI_WAIT);
             ok      = __all_sync(0xffffffffu, ok);
             if (!ok) return false;
@@ -1290,7 +1322,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             const CUtensorMap* mapB = &tmB;
             for (uint32_t w = unit; ok && next_work(cur, c); w += units) {
                 if constexpr (EP) {
-                    if (epp->ragged == RAGGED_K) { // this group's own maps, written by the kernel before this one
+                    if (epp->ragged == RAGGED_K && c.kb1 > c.kb0) { // this group's own maps, written by the kernel before this one
                         mapA = epp->maps + 2u * c.group;
                         mapB = mapA + 1;
                         dep_wait();
@@ -1665,7 +1697,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         if (!ok) break;
                         seen = true;
                     }
-                    TmemPieces<COLUMN_PIECE> pieces{tacc + ch * 32u, NP, false};
+                    TmemPieces<COLUMN_PIECE> pieces{tacc + ch * 32u, NP, c.kb1 == c.kb0};
                     const uint32_t block = epp->ragged == RAGGED_ROWS
                                                ? group_first_block(c.first, c.group, bs) + (col0 - c.first) / bs
                                                : c.z_out * epp->part_blocks + col0 / bs;
@@ -2156,6 +2188,34 @@ __global__ void __launch_bounds__(EPI_THREADS, 1)
                                 const GemmParams p, const EpilogueParams ep)
 {
     gemm_umma_body<BN, OUT, 1, TR, false, true, true>(tmA, tmB, &tmD, tmD, p, &em, &ep);
+}
+
+// A copy of `lines` lines of `length` 16-bit elements with every line padded to `pitch` elements (a
+// multiple of 8) of zeros, for operands whose lines do not start on 16-byte boundaries: TMA
+// addresses the copy.  HBM-bound: (2 length + 2 pitch) bytes per line.
+static __global__ void __launch_bounds__(256)
+    pad_lines_kernel(const uint16_t* src, uint4* dst, uint64_t units, uint32_t length, FastDiv per_line)
+{
+    for (uint64_t u = blockIdx.x * 256ull + threadIdx.x; u < units; u += gridDim.x * 256ull) {
+        uint64_t line;
+        uint32_t at;
+        if (units < 0x80000000ull) {
+            line = fast_div(static_cast<uint32_t>(u), per_line);
+            at   = static_cast<uint32_t>(u) - static_cast<uint32_t>(line) * per_line.d;
+        } else {
+            line = u / per_line.d;
+            at   = static_cast<uint32_t>(u - line * per_line.d);
+        }
+        const uint16_t* from = src + line * length + at * 8u;
+        uint32_t        w[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const uint32_t e  = at * 8u + 2u * k;
+            const uint32_t lo = e < length ? from[2 * k] : 0u, hi = e + 1u < length ? from[2 * k + 1] : 0u;
+            w[k]              = lo | (hi << 16);
+        }
+        dst[u] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
 // Maps of a ragged-K product: group e's copies of the two operands' maps, with the row extent

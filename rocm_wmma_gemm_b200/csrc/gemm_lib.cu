@@ -376,6 +376,7 @@ struct View {
     void*       d;
     uint32_t    M, N, K;
     bool        a_mn, b_mn;
+    uint32_t    a_pitch = 0, b_pitch = 0; // elements between the lines of an operand (0: dense)
 };
 
 static View make_view(const Problem& p)
@@ -627,10 +628,11 @@ static void adapt_config(b200_gemm_config& c, const View& v, size_t batch, int s
 // TMA descriptors
 // ------------------------------------------------------------------------------------------
 static int encode_map(CUtensorMap* tm, CUtensorMapDataType dt, size_t esz, const void* base,
-                      uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b0, uint32_t b1)
+                      uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b0, uint32_t b1, uint64_t pitch = 0)
 {
     const cuuint64_t dims[3]    = {d0, d1, d2};
-    const cuuint64_t strides[2] = {d0 * esz, d0 * d1 * esz};
+    const cuuint64_t line       = pitch ? pitch : d0; // elements from one line to the next
+    const cuuint64_t strides[2] = {line * esz, line * d1 * esz};
     const cuuint32_t box[3]     = {b0, b1, 1};
     const cuuint32_t estr[3]    = {1, 1, 1};
     const CUresult   r = g_encode(tm, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
@@ -645,11 +647,11 @@ static int encode_map(CUtensorMap* tm, CUtensorMapDataType dt, size_t esz, const
 // Operand with MN extent `rows`: K-major -> [batch][rows][K], box 64 x box_rows;
 // MN-major -> [batch][K][rows], box 64 (MN) x 64 (K).
 static int encode_operand(CUtensorMap* tm, bool bf16, const void* base, uint32_t rows, uint32_t K,
-                          size_t batch, bool mn_major, uint32_t box_rows)
+                          size_t batch, bool mn_major, uint32_t box_rows, uint32_t pitch = 0)
 {
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if (!mn_major) return encode_map(tm, dt, 2, base, K, rows, batch, BLOCK_K, box_rows);
-    return encode_map(tm, dt, 2, base, rows, K, batch, 64, BLOCK_K);
+    if (!mn_major) return encode_map(tm, dt, 2, base, K, rows, batch, BLOCK_K, box_rows, pitch);
+    return encode_map(tm, dt, 2, base, rows, K, batch, 64, BLOCK_K, pitch);
 }
 
 // Operand of a one-CTA kernel, `kc` k-blocks per box.
@@ -658,13 +660,14 @@ static int encode_operand(CUtensorMap* tm, bool bf16, const void* base, uint32_t
 //   K-major otherwise: the plain 3-D map, one k-block per box (kc == 1).
 //   MN-major: [batch][K][rows], box 64 (MN) x 64 * kc (K).
 static int encode_operand_slab(CUtensorMap* tm, bool bf16, const void* base, uint32_t rows, uint32_t K,
-                               size_t batch, bool mn_major, uint32_t box_rows, uint32_t kc, bool k4d)
+                               size_t batch, bool mn_major, uint32_t box_rows, uint32_t kc, bool k4d, uint32_t pitch = 0)
 {
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if (mn_major) return encode_map(tm, dt, 2, base, rows, K, batch, 64, BLOCK_K * kc);
-    if (!k4d) return encode_map(tm, dt, 2, base, K, rows, batch, BLOCK_K, box_rows);
+    if (mn_major) return encode_map(tm, dt, 2, base, rows, K, batch, 64, BLOCK_K * kc, pitch);
+    if (!k4d) return encode_map(tm, dt, 2, base, K, rows, batch, BLOCK_K, box_rows, pitch);
+    const cuuint64_t line       = pitch ? pitch : K;
     const cuuint64_t dims[4]    = {(cuuint64_t)BLOCK_K, rows, K / BLOCK_K, batch};
-    const cuuint64_t strides[3] = {(cuuint64_t)K * 2, (cuuint64_t)BLOCK_K * 2, (cuuint64_t)rows * K * 2};
+    const cuuint64_t strides[3] = {line * 2, (cuuint64_t)BLOCK_K * 2, (cuuint64_t)rows * line * 2};
     const cuuint32_t box[4]     = {(cuuint32_t)BLOCK_K, box_rows, kc, 1};
     const cuuint32_t estr[4]    = {1, 1, 1, 1};
     const CUresult   r = g_encode(tm, dt, 4, const_cast<void*>(base), dims, strides, box, estr,
