@@ -299,6 +299,98 @@ static __global__ void __launch_bounds__(32 * SUM_LANES)
 }
 
 // ---------------------------------------------------------------------------------------------
+// Epilogue of a product whose K partitions lie in an f32 workspace: adds them in partition order and
+// applies the epilogue to the sum.  Memory view of C: `lines` lines of `length` contiguous elements
+// per batch item (a multiple of 4).  A block covers `strip` lines x 256 elements: threadIdx.x owns
+// four neighbouring elements, threadIdx.y every fourth line.  Without bias gradients a strip is four
+// lines, one per thread: a thread's loads wait for its stores to the line before.  Bias gradients only
+// where the bias runs along the lines' elements (row-major C): a block's sums are one row of partials.
+// L2-bound: (4 split + sizeof(out) x matrices) bytes per element.
+// ---------------------------------------------------------------------------------------------
+constexpr uint32_t SPLIT_STRIP = 16; // with bias gradients
+
+template <class T>
+__global__ void __launch_bounds__(256)
+    splitk_epilogue_kernel(const float* ws, T* out, const EpilogueParams ep, uint32_t lines, uint32_t length, uint32_t split, uint32_t strip)
+{
+    __shared__ float4 s_sum[4][64];
+    const uint32_t tx = threadIdx.x, ty = threadIdx.y, n = (blockIdx.x * 64u + tx) * 4u;
+    const uint32_t l0 = blockIdx.y * strip, z = blockIdx.z;
+    ptx::grid_dep_wait(); // the partials are complete once the product's grid has finished
+    ptx::grid_dep_launch();
+    const uint64_t item = static_cast<uint64_t>(lines) * length;
+    const float*   part = ws + z * split * item;
+    const T*       bias = static_cast<const T*>(ep.bias) + (ep.bias ? z * ep.bias_stride : 0u);
+    const T*       read = static_cast<const T*>(ep.gradient ? ep.preact : ep.residual);
+    T*             aux  = ep.aux ? static_cast<T*>(ep.preact) : nullptr;
+    float          sum[4] = {};
+    // four elements of C's type
+    struct alignas(4 * sizeof(T)) Four {
+        T v[4];
+    };
+    if (n < length) {
+        float b[4] = {};
+        if (ep.bias && !ep.bias_on_rows)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) b[k] = to_f32(bias[n + k]);
+        for (uint32_t l = l0 + ty; l < min(lines, l0 + strip); l += 4u) {
+            const uint64_t at = static_cast<uint64_t>(l) * length + n, to = z * item + at;
+            float4         a  = *reinterpret_cast<const float4*>(part + at);
+#pragma unroll 4
+            for (uint32_t s = 1; s < split; ++s) {
+                const float4 t = *reinterpret_cast<const float4*>(part + s * item + at);
+                a.x += t.x, a.y += t.y, a.z += t.z, a.w += t.w;
+            }
+            float v[4] = {a.x, a.y, a.z, a.w}, r[4] = {};
+            if (ep.streamed) {
+                const Four f = *reinterpret_cast<const Four*>(read + to);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) r[k] = to_f32(f.v[k]);
+            }
+            Four o;
+            if (ep.gradient) {
+                if (ep.streamed)
+                    with_act(ep.act, [&](auto tag) {
+                        constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] = __fmul_rn(v[k], act_slope<ACT>(r[k], ep));
+                    });
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum[k] += v[k];
+            } else {
+                if (ep.bias && ep.bias_on_rows) b[0] = b[1] = b[2] = b[3] = to_f32(bias[l]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] += b[k];
+                if (aux) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o.v[k] = from_f32<T>(v[k]);
+                    *reinterpret_cast<Four*>(aux + to) = o;
+                }
+                with_act(ep.act, [&](auto tag) {
+                    constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = act_value<ACT>(v[k], ep);
+                });
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] += r[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o.v[k] = from_f32<T>(v[k]);
+            *reinterpret_cast<Four*>(out + to) = o;
+        }
+    }
+    if (!ep.part) return;
+    s_sum[ty][tx] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    __syncthreads();
+    if (ty == 0 && n < length) {
+        float4 t = s_sum[0][tx];
+#pragma unroll
+        for (int y = 1; y < 4; ++y) t.x += s_sum[y][tx].x, t.y += s_sum[y][tx].y, t.z += s_sum[y][tx].z, t.w += s_sum[y][tx].w;
+        *reinterpret_cast<float4*>(ep.part + (static_cast<uint64_t>(z) * ep.part_blocks + blockIdx.y) * length + n) = t;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
 // Backward of an activation where no product precedes it: dZ = dY .* act'(Z), and the sums of dZ
 // over the rows (of the rounded f32 products: no contraction into the sum, so that the sums are the
 // same bits whether dZ is stored or not).  Memory view: `lines` lines of `length` contiguous elements.  Row-major C: a

@@ -1114,8 +1114,14 @@ struct GatherSpec {
     size_t       full_rows, full_cols, row0, col0;
 };
 
+// Takes the place of the reduction pass: launches what turns the f32 K partitions in `ws` (laid out
+// [batch][split][C]) into C.
+struct SplitReduce {
+    virtual cudaError_t launch(const float* ws, uint32_t split, cudaStream_t s) const = 0;
+};
+
 static int launch_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_config* user_cfg, const LaunchEnv& env,
-                       const GatherSpec* gather = nullptr);
+                       const GatherSpec* gather = nullptr, const SplitReduce* reduce = nullptr);
 
 static int run_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_config* user_cfg)
 {
@@ -1138,13 +1144,15 @@ static int run_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_confi
 
 // Plans and launches one (validated, non-empty) problem.
 static int launch_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_config* user_cfg, const LaunchEnv& env,
-                       const GatherSpec* gather)
+                       const GatherSpec* gather, const SplitReduce* reduce)
 {
     int        st;
     const bool fixed = env.ctx == nullptr;
     LaunchPlan pl;
     st = make_plan(p, user_cfg, env.sm_count, &pl);
     if (st != B200_GEMM_OK) return st;
+    if (reduce && (pl.generic || pl.balanced || pl.cluster_k || pl.cfg.split_k <= 1))
+        return fail(B200_GEMM_ERR_BAD_CONFIG, "an epilogue on K partitions needs a plan that has some");
     if (pl.generic && fixed)
         return fail(B200_GEMM_ERR_MISALIGNED,
                     "the allocation-free entry point needs 16-byte aligned pointers and contiguous extents that are "
@@ -1386,7 +1394,7 @@ static int launch_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_co
         const uint64_t mn     = (uint64_t)v.M * v.N;
         const uint64_t total4 = mn * p.batch / 4;
         const unsigned blocks = (unsigned)std::min<uint64_t>((total4 + 255) / 256, (uint64_t)env.sm_count * 8);
-        e = launch_reduce(out, blocks, stream, ws, v.d, mn, split, (uint32_t)p.batch);
+        e = reduce ? reduce->launch(ws, split, stream) : launch_reduce(out, blocks, stream, ws, v.d, mn, split, (uint32_t)p.batch);
         g_launches.fetch_add(1, std::memory_order_relaxed);
         if (ws_stream_ordered) cudaFreeAsync(ws, stream);
         if (e != cudaSuccess) return fail(B200_GEMM_ERR_CUDA, "split-K reduce launch failed: %s", cudaGetErrorString(e));
