@@ -408,18 +408,52 @@ struct ActBackwardParams {
     uint32_t    z0;
 };
 
-// 16 bytes of T.
-template <class T>
+// V neighbouring elements: 16 bytes, or one.
+template <class T, int V>
 struct Pack {
-    static constexpr int N = 16 / sizeof(T);
-    uint4                raw;
-    __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(&raw)[i]); }
-    __device__ __forceinline__ void  set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f32<T>(v); }
+    T v[V];
+    __device__ __forceinline__ void load(const T* from)
+    {
+        if constexpr (V > 1) {
+            static_assert(V * sizeof(T) == 16, "a pack is 16 bytes");
+            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(from));
+            *reinterpret_cast<uint4*>(v) = w;
+        } else {
+            v[0] = *from;
+        }
+    }
+    __device__ __forceinline__ void store(T* to) const
+    {
+        if constexpr (V > 1) __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(v));
+        else *to = v[0];
+    }
 };
+
+// g becomes dZ = g act'(x); its f32 values are added to `sum`.
+template <uint32_t ACT, class T, int V>
+__device__ __forceinline__ void act_backward_pack(Pack<T, V>& g, const Pack<T, V>& x, float (&sum)[V], const EpilogueParams& ep)
+{
+    if constexpr (V > 1) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            float2 v = make_float2(to_f32(g.v[i]), to_f32(g.v[i + 1]));
+            if constexpr (ACT != ACT_NONE) v = __fmul2_rn(v, act_slope<ACT>(make_float2(to_f32(x.v[i]), to_f32(x.v[i + 1])), ep));
+            g.v[i] = from_f32<T>(v.x), g.v[i + 1] = from_f32<T>(v.y);
+            sum[i] += v.x, sum[i + 1] += v.y;
+        }
+    } else {
+        float v = to_f32(g.v[0]);
+        if constexpr (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(x.v[0]), ep));
+        g.v[0] = from_f32<T>(v);
+        sum[0] += v;
+    }
+}
+
+constexpr uint32_t ACT_ROWS = 4; // packs in flight per thread and operand
 
 // Row-major: each thread owns V consecutive columns (V = 16 bytes' worth, or 1 where the rows are
 // not 16-byte aligned) and walks the strip's lines; threads of equal column and different
-// threadIdx.y share a strip and add their sums through shared memory.
+// threadIdx.y share a strip and add their sums through shared memory.  HBM-bound: three matrices.
 template <class T, int V>
 __global__ void __launch_bounds__(256) act_backward_rows_kernel(const ActBackwardParams p, const EpilogueParams ep)
 {
@@ -455,26 +489,24 @@ __global__ void __launch_bounds__(256) act_backward_rows_kernel(const ActBackwar
     if (n < p.length) {
         with_act(ep.act, [&](auto tag) {
             constexpr uint32_t ACT = decltype(tag)::value;
-#pragma unroll 4
-            for (uint32_t r = r0 + ty; r < r1; r += blockDim.y) {
-                const uint64_t at = static_cast<uint64_t>(r) * p.length + n;
-                if constexpr (V > 1) {
-                    Pack<T> g, x, o;
-                    g.raw = __ldcs(reinterpret_cast<const uint4*>(dy + at));
-                    if (ACT != ACT_NONE) x.raw = __ldcs(reinterpret_cast<const uint4*>(z + at));
+            // ACT_ROWS lines' loads before their stores: dZ may be dY or Z, so the compiler cannot move a
+            // later line's loads up by itself
+            for (uint32_t r = r0 + ty; r < r1; r += ACT_ROWS * blockDim.y) {
+                Pack<T, V> g[ACT_ROWS], x[ACT_ROWS];
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        float v = g.get(i);
-                        if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(x.get(i), ep));
-                        o.set(i, v);
-                        sum[i] += v;
+                for (uint32_t k = 0; k < ACT_ROWS; ++k) {
+                    const uint64_t at = static_cast<uint64_t>(r + k * blockDim.y) * p.length + n;
+                    if (r + k * blockDim.y < r1) {
+                        g[k].load(dy + at);
+                        if (ACT != ACT_NONE) x[k].load(z + at);
                     }
-                    if (dz) *reinterpret_cast<uint4*>(dz + at) = o.raw;
-                } else {
-                    float v = to_f32(dy[at]);
-                    if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(z[at]), ep));
-                    if (dz) dz[at] = from_f32<T>(v);
-                    sum[0] += v;
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < ACT_ROWS; ++k) {
+                    if (r + k * blockDim.y < r1) {
+                        act_backward_pack<ACT>(g[k], x[k], sum, ep);
+                        if (dz) g[k].store(dz + static_cast<uint64_t>(r + k * blockDim.y) * p.length + n);
+                    }
                 }
             }
         });
@@ -506,30 +538,29 @@ __global__ void __launch_bounds__(256) act_backward_cols_kernel(const ActBackwar
     const T*       z    = p.z ? static_cast<const T*>(p.z) + base : nullptr;
     T*             dz   = p.dz ? static_cast<T*>(p.dz) + base : nullptr;
     float          sum  = 0.f;
+    float          sums[V] = {};
     with_act(ep.act, [&](auto tag) {
         constexpr uint32_t ACT = decltype(tag)::value;
-#pragma unroll 4
-        for (uint32_t i0 = e0 + lane * V; i0 < e1; i0 += 32u * V) {
-            if constexpr (V > 1) {
-                Pack<T> g, x, o;
-                g.raw = __ldcs(reinterpret_cast<const uint4*>(dy + i0));
-                if (ACT != ACT_NONE) x.raw = __ldcs(reinterpret_cast<const uint4*>(z + i0));
+        for (uint32_t i0 = e0 + lane * V; i0 < e1; i0 += ACT_ROWS * 32u * V) {
+            Pack<T, V> g[ACT_ROWS], x[ACT_ROWS];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float v = g.get(i);
-                    if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(x.get(i), ep));
-                    o.set(i, v);
-                    sum += v;
+            for (uint32_t k = 0; k < ACT_ROWS; ++k) {
+                if (i0 + k * 32u * V < e1) {
+                    g[k].load(dy + i0 + k * 32u * V);
+                    if (ACT != ACT_NONE) x[k].load(z + i0 + k * 32u * V);
                 }
-                if (dz) *reinterpret_cast<uint4*>(dz + i0) = o.raw;
-            } else {
-                float v = to_f32(dy[i0]);
-                if (ACT != ACT_NONE) v = __fmul_rn(v, act_slope<ACT>(to_f32(z[i0]), ep));
-                if (dz) dz[i0] = from_f32<T>(v);
-                sum += v;
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < ACT_ROWS; ++k) {
+                if (i0 + k * 32u * V < e1) {
+                    act_backward_pack<ACT>(g[k], x[k], sums, ep);
+                    if (dz) g[k].store(dz + i0 + k * 32u * V);
+                }
             }
         }
     });
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum += sums[i];
     if (!ep.part) return;
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
