@@ -67,6 +67,10 @@ cudaError_t launch_one(const EpilogueLaunch& l, cudaStream_t s)
 
 cudaError_t set_epilogue_attributes()
 {
+    cudaFuncAttributes a; // (loads the kernels that need no attribute)
+    cudaError_t        r = cudaFuncGetAttributes(&a, pad_lines_kernel);
+    if (r == cudaSuccess) r = cudaFuncGetAttributes(&a, ragged_maps_kernel);
+    if (r != cudaSuccess) return r;
     cudaError_t e = set_one<64, 1, false, false>();
     if (e == cudaSuccess) e = set_one<128, 1, false, false>();
     if (e == cudaSuccess) e = set_one<256, 1, false, false>();
@@ -114,12 +118,12 @@ cudaError_t launch_epilogue_gemm(const EpilogueLaunch& l, cudaStream_t s)
     return cudaErrorInvalidValue; // not a compiled width
 }
 
-cudaError_t epilogue_pairs(int bn, uint32_t smem, int* pairs)
+cudaError_t epilogue_pairs(int* pairs)
 {
     cudaLaunchConfig_t q = {};
     q.gridDim            = dim3(2 * 148);
     q.blockDim           = dim3(EPI_THREADS);
-    q.dynamicSmemBytes   = smem;
+    q.dynamicSmemBytes   = epilogue_smem_limit(OUT_F32);
     cudaLaunchAttribute a[1];
     a[0].id               = cudaLaunchAttributeClusterDimension;
     a[0].val.clusterDim.x = 2;
@@ -127,8 +131,7 @@ cudaError_t epilogue_pairs(int bn, uint32_t smem, int* pairs)
     a[0].val.clusterDim.z = 1;
     q.attrs               = a;
     q.numAttrs            = 1;
-    return bn == 512 ? cudaOccupancyMaxActiveClusters(pairs, gemm_epilogue_kernel<512, OUT_F32, 2>, &q)
-                     : cudaOccupancyMaxActiveClusters(pairs, gemm_epilogue_kernel<256, OUT_F32, 2>, &q);
+    return cudaOccupancyMaxActiveClusters(pairs, gemm_epilogue_kernel<256, OUT_F32, 2>, &q);
 }
 
 cudaError_t launch_pad_lines(const void* src, void* dst, uint64_t lines, uint32_t length, uint32_t pitch, const FastDiv& per_line, int sm_count, cudaStream_t s)

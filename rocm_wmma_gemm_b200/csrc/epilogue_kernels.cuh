@@ -20,10 +20,11 @@ struct EpilogueLaunch {
     EpilogueParams ep;
 };
 
+// Shared-memory opt-in of every kernel here; loads them too.
 cudaError_t set_epilogue_attributes();
 cudaError_t launch_epilogue_gemm(const EpilogueLaunch& l, cudaStream_t s);
-// CTA pairs of the kernel that can be resident at once.
-cudaError_t epilogue_pairs(int bn, uint32_t smem, int* pairs);
+// CTA pairs that can be resident at once.
+cudaError_t epilogue_pairs(int* pairs);
 // Lines of `length` 16-bit elements copied to lines of `pitch` elements, zero-padded.
 cudaError_t launch_pad_lines(const void* src, void* dst, uint64_t lines, uint32_t length, uint32_t pitch, const FastDiv& per_line, int sm_count, cudaStream_t s);
 cudaError_t launch_ragged_maps(const CUtensorMap& a, const CUtensorMap& b, CUtensorMap* maps, const int32_t* offsets, uint32_t groups,

@@ -1322,8 +1322,8 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             const CUtensorMap* mapB = &tmB;
             for (uint32_t w = unit; ok && next_work(cur, c); w += units) {
                 if constexpr (EP) {
-                    if (epp->ragged == RAGGED_K && c.kb1 > c.kb0) { // this group's own maps, written by the kernel before this one
-                        mapA = epp->maps + 2u * c.group;
+                    if (epp->ragged == RAGGED_K && c.kb1 > c.kb0 && mapA != epp->maps + 2u * c.group) {
+                        mapA = epp->maps + 2u * c.group; // this group's own maps, written by the kernel before this one
                         mapB = mapA + 1;
                         dep_wait();
                         ptx::fence_tensormap_acquire(mapA);

@@ -165,7 +165,7 @@ struct DeviceCtx {
     std::atomic<bool> ready{false}; // set last, read first: initialised contexts skip the lock
     int           sm_count = 0;
     PairCache     pairs;
-    PairCache     epilogue_pairs; // of the kernels with an epilogue (tile_n up to 256 / 512)
+    int           epilogue_pairs = 0; // co-resident CTA pairs of the kernels with an epilogue
     unsigned int* d_status = nullptr;
     // split-K workspaces, one per stream that has used split-K (calls on one stream are ordered,
     // so they can share a buffer; calls on different streams must not - and two host threads
@@ -175,6 +175,7 @@ struct DeviceCtx {
         float*       ptr;
         size_t       bytes;
         int          kind; // WS_SPLIT_K or WS_EPILOGUE: a call may use one of each
+        const void*  thread; // the per-thread default stream is one handle for many streams: whose (else nullptr)
     };
     std::vector<Workspace> workspaces;
     // buffers a workspace has outgrown: freed once the work that was queued on them has drained
@@ -269,6 +270,8 @@ static cudaError_t set_all_kernel_attributes()
     return e;
 }
 
+static int prepare_epilogues(DeviceCtx* ctx); // epilogue_driver.inc
+
 static int get_ctx(DeviceCtx** out)
 {
     int         dev = -1;
@@ -302,7 +305,8 @@ static int get_ctx(DeviceCtx** out)
         CUDA_TRY(cudaMalloc(&c.d_status, sizeof(unsigned int)));
         CUDA_TRY(cudaMemset(c.d_status, 0, sizeof(unsigned int)));
         CUDA_TRY(set_all_kernel_attributes());
-        CUDA_TRY(set_epilogue_attributes());
+        const int st = prepare_epilogues(&c);
+        if (st != B200_GEMM_OK) return st;
         c.ready.store(true, std::memory_order_release);
     }
     *out = &c;
@@ -315,6 +319,8 @@ static int get_ctx(DeviceCtx** out)
 // use it - but retired behind an event and freed by a later call once that event has passed.
 static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, float** out, int kind = WS_SPLIT_K)
 {
+    static thread_local char t_self;
+    const void* const        thread = stream == cudaStreamPerThread ? &t_self : nullptr;
     std::lock_guard<std::mutex> lock(ctx->ws_mutex);
     for (size_t i = 0; i < ctx->retired.size();) {
         if (cudaEventQuery(ctx->retired[i].drained) == cudaSuccess) {
@@ -328,7 +334,7 @@ static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, floa
         }
     }
     for (auto& w : ctx->workspaces) {
-        if (w.stream != stream || w.kind != kind) continue;
+        if (w.stream != stream || w.kind != kind || w.thread != thread) continue;
         if (w.bytes < bytes) {
             const size_t want  = bytes + bytes / 4;
             float*       fresh = nullptr;
@@ -349,7 +355,7 @@ static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, floa
         *out = w.ptr;
         return B200_GEMM_OK;
     }
-    DeviceCtx::Workspace w{stream, nullptr, 0, kind};
+    DeviceCtx::Workspace w{stream, nullptr, 0, kind, thread};
     CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&w.ptr), bytes));
     w.bytes = bytes;
     ctx->workspaces.push_back(w);
@@ -1121,7 +1127,7 @@ struct SplitReduce {
 };
 
 static int launch_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_config* user_cfg, const LaunchEnv& env,
-                       const GatherSpec* gather = nullptr, const SplitReduce* reduce = nullptr);
+                       const GatherSpec* gather = nullptr, const SplitReduce* reduce = nullptr, const LaunchPlan* planned = nullptr);
 
 static int run_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_config* user_cfg)
 {
@@ -1144,13 +1150,17 @@ static int run_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_confi
 
 // Plans and launches one (validated, non-empty) problem.
 static int launch_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_config* user_cfg, const LaunchEnv& env,
-                       const GatherSpec* gather, const SplitReduce* reduce)
+                       const GatherSpec* gather, const SplitReduce* reduce, const LaunchPlan* planned)
 {
     int        st;
     const bool fixed = env.ctx == nullptr;
     LaunchPlan pl;
-    st = make_plan(p, user_cfg, env.sm_count, &pl);
-    if (st != B200_GEMM_OK) return st;
+    if (planned) {
+        pl = *planned;
+    } else {
+        st = make_plan(p, user_cfg, env.sm_count, &pl);
+        if (st != B200_GEMM_OK) return st;
+    }
     if (reduce && (pl.generic || pl.balanced || pl.cluster_k || pl.cfg.split_k <= 1))
         return fail(B200_GEMM_ERR_BAD_CONFIG, "an epilogue on K partitions needs a plan that has some");
     if (pl.generic && fixed)

@@ -120,6 +120,52 @@ def test_fused_tiles(L, M, N, K, pair, layouts):
     fused(L, M, N, K, pair, layouts, act="none", grad=True)
 
 
+@pytest.mark.parametrize("M,N,K,layouts,pair", [
+    (16, 64, 64, (1, 0, 0), "bf16"), (16, 64, 2048, (1, 0, 0), "bf16"), (32, 64, 2048, (1, 0, 0), "f16"),      # narrow tiles, K partitions in the workspace
+    (16, 64, 2048, (0, 0, 0), "bf16"), (192, 512, 8192, (0, 0, 0), "bf16"), (192, 1024, 8192, (0, 0, 0), "f16"),
+    (192, 8192, 64, (0, 0, 0), "bf16"), (512, 8192, 64, (0, 0, 0), "bf16"),                                     # 128 x 128 and 128 x 256 tiles
+    (100, 4096, 4096, (1, 0, 0), "f32"), (192, 8192, 4096, (0, 0, 0), "bf16"),                                  # K partitions in clusters
+    (192, 8192, 2048, (0, 0, 1), "f32"), (192, 4096, 4096, (0, 0, 1), "bf16"), (512, 8192, 2048, (0, 0, 1), "f32"),  # CTA pairs, widths 160 to 224
+    (512, 8192, 1024, (0, 0, 1), "bf16"), (1024, 8192, 1024, (0, 0, 0), "bf16"), (1024, 8192, 1024, (0, 0, 0), "f32"),  # 256 and 512 wide
+    (16, 128, 64, (0, 0, 0), "bf16"), (16, 128, 2048, (0, 0, 0), "bf16"), (48, 128, 2048, (0, 0, 0), "f32"),    # operands swapped
+    (16, 512, 2048, (0, 0, 1), "bf16"), (32, 512, 2048, (0, 0, 1), "f32"), (256, 64, 2048, (1, 0, 0), "bf16"),  # and K partitions in clusters
+    (16, 256, 0, (0, 0, 1), "bf16"), (300, 256, 0, (1, 0, 0), "f32"), (2048, 1024, 0, (0, 0, 0), "bf16"),
+])
+def test_fused_every_kernel(L, M, N, K, layouts, pair):
+    """Every kernel the plan can choose, each mode of the epilogue."""
+    p = (pair, "bf16" if pair != "f16" else "f16")
+    for i, act in enumerate(("gelu", "none", "silu")):
+        fused(L, M, N, K, p, layouts, act=act, residual=i != 1, preact=i != 2, seed=i)
+        fused(L, M, N, K, p, layouts, act=act, residual=False, bias=i != 0, preact=False, seed=i)
+        fused(L, M, N, K, p, layouts, act=act, grad=True, bias_grad=i != 1, seed=i)
+    fused(L, M, N, K, p, layouts, act="relu", in_place=True, offset=1)  # C, residual and Z between 16-byte boundaries
+    fused(L, M, N, K, p, layouts, act="relu", in_place=True, grad=True, offset=1)
+
+
+def test_past_32_bits(L):
+    """Matrices of more than 2^31 elements: rows from both ends and the middle."""
+    M, N, K = 66000, 32776, 64
+    gen = make_gen("large")
+    bf = torch.bfloat16
+    a, b = randn(gen, M, K, dtype=bf), randn(gen, N, K, dtype=bf, scale=K ** -0.5)
+    c = torch.randn(M * N // 8, device="cuda", generator=gen).to(bf).repeat(8).view(M, N)
+    rows = torch.tensor([0, 1, 127, 128, M // 2, 65535, 65536, M - 130, M - 1], device="cuda")
+    res, bias = c[rows].clone(), randn(gen, N, dtype=bf)
+    L.gemm_fused(c, a, b, M, N, K, layout_b=1, activation="silu", bias=bias, residual=c)
+    y, ey, _, _ = forward(a[rows], b.t(), "silu", bias, res)
+    check(c[rows], y, ey, "fused")
+    # the same rows as four groups (weights shared by copying), gradient in place with bias sums
+    offs, T, spans = ragged([1000, 64000, 0, 1000])
+    w = b.repeat(4, 1, 1)
+    z, bg = c[rows].clone(), torch.empty(4, N, device="cuda")
+    L.gemm_grouped(c, a, w, offs, T, N, K, 4, layout_b=1, activation="silu", preact=c, gradient=True, bias_grad=bg)
+    d, ed = gradient(*product(a[rows], b.t()), z, "silu")
+    check(c[rows], d, ed, "grouped")
+    dz, s = c[rows].clone(), torch.empty(N, device="cuda")
+    L.activation_backward(c, c, c, M, N, activation="relu", bias_grad=s)
+    check(c[rows], *gradient(dz.double(), torch.zeros(len(rows), N, device="cuda", dtype=torch.float64), dz, "relu"), "backward")
+
+
 def test_fused_in_place(L):
     for M, N, K in [(16, 512, 256), (300, 520, 264), (7, 9, 11)]:
         for pair in PAIRS:
@@ -380,6 +426,18 @@ def test_wgrad_neighbours_with_infinities(L):
     assert torch.isnan(c[1]).any()
 
 
+def test_wgrad_without_rows(L):
+    offs = torch.zeros(4, dtype=torch.int32, device="cuda")
+    a = torch.empty(0, 72, device="cuda", dtype=torch.bfloat16)
+    for lc in (0, 1):
+        c = Guarded((3, 72, 136), torch.float32)
+        L.gemm_grouped_wgrad(c.t, a, a, offs, 0, 72, 136, 3, layout_c=lc)
+        assert (c.t == 0).all() and c.intact()
+        c.t.fill_(5)
+        L.gemm_grouped_wgrad(c.t, a, a, offs, 0, 72, 136, 3, layout_c=lc, accumulate=True)
+        assert (c.t == 5).all()
+
+
 def test_wgrad_unaligned(L):
     wgrad(L, COUNTS["ragged"], 72, 136, offset=1)
     wgrad(L, COUNTS["ragged"], 72, 136, ("f32", "f16"), lc=1, offset=4, accumulate=True)
@@ -637,6 +695,34 @@ def test_graphs_replay_and_do_not_share_scratch(L):
             _grad_check(s)
         for e, (p, q) in enumerate(spans):
             check(gc[e], *product(ga[p:q].t(), gb[p:q]))
+
+
+def test_two_host_threads(L):
+    """Calls from two threads, each on its own stream."""
+    import threading
+    gen = make_gen("threads")
+    sets = [_work_set(gen, M=500 + 100 * i, N=1032, K=2056) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(s, st):
+        try:
+            with torch.cuda.stream(st):
+                for _ in range(40):
+                    _grad_call(L, s)
+        except Exception as e:  # noqa: BLE001 (reported below)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(sets, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for s in sets:
+        _grad_check(s)
 
 
 def test_results_repeat_bit_for_bit(L):
