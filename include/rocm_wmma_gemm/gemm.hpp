@@ -127,6 +127,166 @@ void gemm(T* C, U* A, U* B, size_t M, size_t N, size_t K, hipStream_t& stream)
     gemm<layout_C, layout_A, layout_B>(C, A, B, M, N, K, 1, stream);
 }
 
+// Products with epilogues, grouped products and their gradients: forwards to the C ABI, whose header
+// has the rules (b200_gemm_fused and the entry points after it).  No counterpart in the reference.
+
+enum class activation
+{
+    none      = B200_GEMM_ACT_NONE,
+    relu      = B200_GEMM_ACT_RELU,
+    silu      = B200_GEMM_ACT_SILU,
+    gelu_tanh = B200_GEMM_ACT_GELU_TANH,
+    gelu      = B200_GEMM_ACT_GELU
+};
+
+// What surrounds a product with output type T; the members are those of b200_gemm_epilogue.
+template<class T>
+struct epilogue
+{
+    activation act         = activation::none;
+    bool       gradient    = false;
+    const T*   bias        = nullptr;
+    const T*   residual    = nullptr;
+    T*         preact      = nullptr;
+    float*     bias_grad   = nullptr;
+    size_t     bias_stride = 0;
+
+    b200_gemm_epilogue abi() const
+    {
+        return {static_cast<int>(act), gradient ? 1 : 0, bias, residual, preact, bias_grad, bias_stride};
+    }
+};
+
+namespace detail
+{
+
+inline void check(int status, const char* name)
+{
+    if(status != B200_GEMM_OK)
+        throw std::runtime_error(std::string("rocm_wmma_gemm::") + name + ": " + b200_gemm_last_error());
+}
+
+} // namespace detail
+
+// C = act(A*B + bias) + residual, or with gradient set C = (A*B) .* act'(preact) and its column sums.
+template<m_layout layout_C, m_layout layout_A, m_layout layout_B, class T, class U>
+void gemm_fused(T*                 C,
+                const U*           A,
+                const U*           B,
+                size_t             M,
+                size_t             N,
+                size_t             K,
+                size_t             batch_count,
+                const epilogue<T>& e,
+                hipStream_t&       stream)
+{
+    const b200_gemm_epilogue epi = e.abi();
+    detail::check(b200_gemm_fused(detail::type_index<T, U>(),
+                                  C,
+                                  A,
+                                  B,
+                                  M,
+                                  N,
+                                  K,
+                                  batch_count,
+                                  static_cast<int>(layout_C),
+                                  static_cast<int>(layout_A),
+                                  static_cast<int>(layout_B),
+                                  &stream,
+                                  &epi),
+                  "gemm_fused");
+}
+
+// Rows [offsets[e], offsets[e+1]) of A (rows x K) times matrix e of B, into the same rows of C.
+template<m_layout layout_B, class T, class U>
+void gemm_grouped(T*                 C,
+                  const U*           A,
+                  const U*           B,
+                  const int*         offsets,
+                  size_t             rows,
+                  size_t             N,
+                  size_t             K,
+                  size_t             groups,
+                  const epilogue<T>& e,
+                  hipStream_t&       stream)
+{
+    const b200_gemm_epilogue epi = e.abi();
+    detail::check(b200_gemm_grouped(detail::type_index<T, U>(),
+                                    C,
+                                    A,
+                                    B,
+                                    offsets,
+                                    rows,
+                                    N,
+                                    K,
+                                    groups,
+                                    static_cast<int>(layout_B),
+                                    &stream,
+                                    &epi),
+                  "gemm_grouped");
+}
+
+// C_e = A[rows of e]^T * B[rows of e] for every group, added to C_e with `accumulate`.
+template<m_layout layout_C, class T, class U>
+void gemm_grouped_wgrad(T*           C,
+                        const U*     A,
+                        const U*     B,
+                        const int*   offsets,
+                        size_t       rows,
+                        size_t       M,
+                        size_t       N,
+                        size_t       groups,
+                        bool         accumulate,
+                        hipStream_t& stream)
+{
+    detail::check(b200_gemm_grouped_wgrad(detail::type_index<T, U>(),
+                                          C,
+                                          A,
+                                          B,
+                                          offsets,
+                                          rows,
+                                          M,
+                                          N,
+                                          groups,
+                                          static_cast<int>(layout_C),
+                                          accumulate ? 1 : 0,
+                                          &stream),
+                  "gemm_grouped_wgrad");
+}
+
+// dZ = dY .* act'(preact) for M x N matrices, and the column sums of dZ (offsets: rows in groups, else nullptr).
+template<m_layout layout, class T>
+void activation_backward(T*           dZ,
+                         const T*     dY,
+                         const T*     preact,
+                         size_t       M,
+                         size_t       N,
+                         size_t       batch_count,
+                         activation   act,
+                         float*       bias_grad,
+                         size_t       bias_stride,
+                         const int*   offsets,
+                         size_t       groups,
+                         hipStream_t& stream)
+{
+    using U = std::conditional_t<std::is_same_v<T, half>, half, __hip_bfloat16>; // any pair with this output type
+    detail::check(b200_gemm_activation_backward(detail::type_index<T, U>(),
+                                                dZ,
+                                                dY,
+                                                preact,
+                                                M,
+                                                N,
+                                                batch_count,
+                                                static_cast<int>(layout),
+                                                static_cast<int>(act),
+                                                bias_grad,
+                                                bias_stride,
+                                                offsets,
+                                                groups,
+                                                &stream),
+                  "activation_backward");
+}
+
 } // namespace rocm_wmma_gemm
 
 #endif // ROCM_WMMA_GEMM_GEMM_HPP

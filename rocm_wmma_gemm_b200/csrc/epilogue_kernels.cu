@@ -79,7 +79,6 @@ cudaError_t set_epilogue_attributes()
     if (e == cudaSuccess) e = set_one<16, 1, true, false>();
     if (e == cudaSuccess) e = set_one<32, 1, true, false>();
     if (e == cudaSuccess) e = set_one<64, 1, true, false>();
-    if (e == cudaSuccess) e = set_one<128, 1, true, false>();
     if (e == cudaSuccess) e = set_one<128, 1, false, true>();
     if (e == cudaSuccess) e = set_one<256, 1, false, true>();
     if (e == cudaSuccess) e = set_one<16, 1, true, true>();
@@ -96,7 +95,6 @@ cudaError_t launch_epilogue_gemm(const EpilogueLaunch& l, cudaStream_t s)
             case 16: return ks ? launch_one<16, 1, true, true>(l, s) : launch_one<16, 1, true, false>(l, s);
             case 32: return ks ? launch_one<32, 1, true, true>(l, s) : launch_one<32, 1, true, false>(l, s);
             case 64: return ks ? launch_one<64, 1, true, true>(l, s) : launch_one<64, 1, true, false>(l, s);
-            case 128: return ks ? cudaErrorInvalidValue : launch_one<128, 1, true, false>(l, s);
         }
     } else if (ks) {
         switch (l.bn) {

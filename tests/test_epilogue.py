@@ -1,6 +1,9 @@
 """CPU tests of the products with epilogues and the grouped products: what the entry points
 refuse before anything could run, and how the Python view names them."""
 import ctypes
+import os
+import shutil
+import subprocess
 
 import pytest
 
@@ -136,3 +139,23 @@ def test_python_names(gl):
         L.gemm_fused(C, A, B, 8, 8, 8, activation="swish", types=2)
     with pytest.raises(g.GemmError):
         L.gemm_fused(C, A, B, 8, 8, 8, activation="gelu", gradient=True, types=2)
+
+
+CPP = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp")
+
+
+@pytest.fixture(scope="session")
+def frontend(gemm_lib):
+    if shutil.which("g++") is None:
+        pytest.skip("no g++")
+    return subprocess.run(["sh", os.path.join(CPP, "build_epilogue_test.sh")], check=True, capture_output=True, text=True).stdout.strip()
+
+
+def test_cpp_front_end_compiles(frontend):
+    assert os.path.exists(frontend)
+
+
+@pytest.mark.gpu
+def test_cpp_front_end(frontend):
+    r = subprocess.run([frontend], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
