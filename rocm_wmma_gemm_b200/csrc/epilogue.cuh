@@ -216,37 +216,63 @@ __device__ __forceinline__ uint32_t group_first_block(uint32_t first_row, uint32
     return first_row / part_rows + e;
 }
 
+// Walks the groups in order, 32 at a time, by one warp: f(g, lo, hi) for group g = this lane's of the 32,
+// with its sanitised rows [lo, hi) (empty past the last group); stops when f returns true.  The
+// offsets of GROUP_BATCH x 32 groups are loaded together, so that their latencies overlap.
+constexpr uint32_t GROUP_BATCH = 4;
+
+template <class F>
+__device__ __forceinline__ void for_each_group(const int32_t* offsets, uint32_t groups, uint32_t rows, F&& f)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t       top  = clamp_offset(offsets[0], rows); // running maximum up to the first of the 32
+    for (uint32_t b0 = 0; b0 < groups; b0 += 32u * GROUP_BATCH) {
+        uint32_t end[GROUP_BATCH];
+#pragma unroll
+        for (uint32_t i = 0; i < GROUP_BATCH; ++i) {
+            const uint32_t g = b0 + i * 32u + lane;
+            end[i]           = g < groups ? clamp_offset(offsets[g + 1u], rows) : 0u;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < GROUP_BATCH; ++i) {
+            if (b0 + i * 32u >= groups) return;
+            const uint32_t hi = max(warp_scan_max(end[i], lane), top);
+            uint32_t       lo = __shfl_up_sync(0xffffffffu, hi, 1);
+            if (lane == 0) lo = top;
+            if (f(b0 + i * 32u + lane, lo, hi)) return;
+            top = __shfl_sync(0xffffffffu, hi, 31);
+        }
+    }
+}
+
 // The group and rows of row-tile number `want` (tiles of `tile` rows, groups in order); the whole
 // warp takes part.  False when there are fewer tiles.
 __device__ __forceinline__ bool locate_row_tile(const int32_t* offsets, uint32_t groups, uint32_t rows,
                                                 uint32_t tile, uint32_t want, uint32_t& e, uint32_t& first,
                                                 uint32_t& row0, uint32_t& row1)
 {
-    const uint32_t lane = threadIdx.x & 31u;
-    uint32_t       top = 0u, before = 0u; // running maximum of the offsets, tiles of the groups so far
-    for (uint32_t g0 = 0; g0 < groups; g0 += 32u) {
-        const uint32_t g  = g0 + lane;
-        uint32_t       lo = g < groups ? clamp_offset(offsets[g], rows) : 0u;
-        uint32_t       hi = g < groups ? clamp_offset(offsets[g + 1u], rows) : 0u;
-        lo = max(warp_scan_max(lo, lane), top);
-        hi = max(warp_scan_max(hi, lane), lo);
-        const uint32_t tiles = g < groups ? (hi - lo + tile - 1u) / tile : 0u;
+    const uint32_t lane   = threadIdx.x & 31u;
+    uint32_t       before = 0u; // tiles of the groups so far
+    bool           found  = false;
+    for_each_group(offsets, groups, rows, [&](uint32_t g, uint32_t lo, uint32_t hi) {
+        const uint32_t tiles = (hi - lo + tile - 1u) / tile;
         const uint32_t incl  = before + warp_scan_add(tiles, lane);
         const uint32_t hit   = __ballot_sync(0xffffffffu, want < incl);
         if (hit) {
-            const int src = __ffs(hit) - 1;
-            e             = g0 + src;
-            first         = __shfl_sync(0xffffffffu, lo, src);
+            const int src      = __ffs(hit) - 1;
+            e                  = __shfl_sync(0xffffffffu, g, src);
+            first              = __shfl_sync(0xffffffffu, lo, src);
             const uint32_t end = __shfl_sync(0xffffffffu, hi, src);
             const uint32_t tb  = __shfl_sync(0xffffffffu, incl - tiles, src);
             row0               = first + (want - tb) * tile;
             row1               = min(end, row0 + tile);
+            found              = true;
             return true;
         }
-        top    = __shfl_sync(0xffffffffu, hi, 31);
         before = __shfl_sync(0xffffffffu, incl, 31);
-    }
-    return false;
+        return false;
+    });
+    return found;
 }
 
 // Rows [lo, hi) of group e; the whole warp takes part.
@@ -255,6 +281,7 @@ __device__ __forceinline__ void group_rows(const int32_t* offsets, uint32_t e, u
 {
     const uint32_t lane = threadIdx.x & 31u;
     uint32_t       top  = 0u;
+#pragma unroll 8
     for (uint32_t g = lane; g <= e; g += 32u) top = max(top, clamp_offset(offsets[g], rows));
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));

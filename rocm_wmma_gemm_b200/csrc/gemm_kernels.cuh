@@ -399,22 +399,18 @@ struct GroupTable {
 __device__ __forceinline__ void build_group_table(const EpilogueParams& ep, uint32_t tile, uint32_t* first, uint32_t* tiles)
 {
     const uint32_t lane = threadIdx.x & 31u;
-    uint32_t       top = 0u, before = 0u;
-    for (uint32_t g0 = 0; g0 <= ep.groups; g0 += 32u) {
-        const uint32_t g = g0 + lane;
-        const uint32_t v = g <= ep.groups ? clamp_offset(ep.offsets[g], ep.rows) : 0u;
-        const uint32_t m = max(warp_scan_max(v, lane), top); // first row of group g
-        uint32_t       prev = __shfl_up_sync(0xffffffffu, m, 1);
-        if (lane == 0) prev = g0 ? top : m;
-        const uint32_t n    = (m - prev + tile - 1u) / tile; // tiles of group g - 1
-        const uint32_t incl = before + warp_scan_add(n, lane);
-        if (g <= ep.groups) {
-            first[g] = m;
-            tiles[g] = incl;
+    uint32_t       before = 0u;
+    if (lane == 0) tiles[0] = 0u;
+    for_each_group(ep.offsets, ep.groups, ep.rows, [&](uint32_t g, uint32_t lo, uint32_t hi) {
+        const uint32_t incl = before + warp_scan_add((hi - lo + tile - 1u) / tile, lane);
+        if (g < ep.groups) {
+            first[g]      = lo;
+            tiles[g + 1u] = incl;
+            if (g + 1u == ep.groups) first[ep.groups] = hi;
         }
-        top    = __shfl_sync(0xffffffffu, m, 31);
         before = __shfl_sync(0xffffffffu, incl, 31);
-    }
+        return false;
+    });
 }
 
 // tile_coords with the divisors the host has prepared.

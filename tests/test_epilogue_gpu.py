@@ -764,3 +764,13 @@ def test_python_refusals(L):
     with pytest.raises(g.GemmError):
         L.gemm_fused(a, a, c, 64, 64, 64)  # C is A
     assert (c == 0).all() and (a == 0).all()
+
+
+def test_same_sizes_in_turn(L):
+    """One size in all its modes, alignments, layouts and types, in changing order: no call runs by another's plan."""
+    cases = [dict(pair=p, layouts=l, offset=o, grad=gr, residual=r, preact=z, act="silu", batch=n)
+             for p in PAIRS for l in ((0, 0, 1), (1, 1, 0)) for o in (0, 1, 4) for gr, r, z in
+             ((False, True, True), (False, False, False), (False, True, False), (True, True, True)) for n in (1, 2)]
+    for step in (1, 59, 101):  # (each without a common factor with the number of cases)
+        for i in range(len(cases)):
+            fused(L, 128, 256, 1024, **cases[i * step % len(cases)])
