@@ -15,7 +15,9 @@
  *     read with b200_gemm_last_status() / b200_gemm_last_error().
  *
  *  2. `b200_gemm_*` twins that return a status code, plus helpers the reference does not
- *     have (host-buffer call, explicit config, column-slab partition, device status).
+ *     have (host-buffer call, explicit config, column-slab partition, device status), and the
+ *     products with epilogues, grouped products and their gradients (b200_gemm_fused and the
+ *     entry points after it).
  *
  * All pointers named C/A/B in group 1 and in b200_gemm_<out>_<in> are DEVICE pointers.
  * `stream` is a POINTER TO a cudaStream_t (the reference passes `&stream`); NULL means
