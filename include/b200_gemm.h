@@ -274,7 +274,7 @@ int b200_gemm_slab_host(b200_gemm_comm* comm, int types, void* C_slab, const voi
  * graph after the first call on the device.  A call that needs scratch memory (bias gradients, K
  * partitions, operands that have to be padded) keeps it per stream and lets it grow on demand; a
  * captured call's scratch belongs to the graph.  Calls that overlap on the GPU must not share
- * outputs; host threads must not issue calls on one stream at the same time.
+ * outputs.  Host threads may use one stream: calls that need scratch memory queue one after the other.
  *
  * Refused before anything runs: bad layouts, sizes, activations (BAD_LAYOUT, BAD_SIZE, BAD_CONFIG),
  * missing pointers (NULL_POINTER), pointers not aligned to their element (MISALIGNED), a bias,

@@ -168,8 +168,9 @@ struct DeviceCtx {
     int           epilogue_pairs = 0; // co-resident CTA pairs of the kernels with an epilogue
     unsigned int* d_status = nullptr;
     // split-K workspaces, one per stream that has used split-K (calls on one stream are ordered,
-    // so they can share a buffer; calls on different streams must not - and two host threads
-    // must not issue calls on the same stream at the same time)
+    // so they can share a buffer; calls on different streams must not).  A call holds its stream's lock
+    // from taking a workspace to its last launch on it: the launches of two host threads that use
+    // one stream do not mix, nor does a buffer go that the other has yet to launch on.
     struct Workspace {
         cudaStream_t stream;
         float*       ptr;
@@ -185,6 +186,11 @@ struct DeviceCtx {
     };
     std::vector<Retired> retired;
     std::mutex           ws_mutex;   // guards workspaces / retired
+    std::recursive_mutex stream_mutex[16]; // by stream (a call may take a workspace of each kind)
+    std::unique_lock<std::recursive_mutex> lock_stream(cudaStream_t s)
+    {
+        return std::unique_lock<std::recursive_mutex>(stream_mutex[(reinterpret_cast<uintptr_t>(s) >> 4) % 16]);
+    }
     std::mutex           host_mutex; // held for the whole of a host-buffer call
     // host-buffer path: compute stream, copy-in / copy-out streams and the events chaining them
     cudaStream_t h_in = nullptr, h_out = nullptr;
@@ -1277,6 +1283,7 @@ static int launch_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_co
     const size_t ws_bytes = balanced ? ws_slots * tile_rows * bn * sizeof(float)
                                      : (split > 1 && !cluster_k ? (size_t)p.batch * split * v.M * v.N * sizeof(float) : 0);
     bool         ws_stream_ordered = false;
+    std::unique_lock<std::recursive_mutex> ws_lock; // (to the end of this function)
     if ((split > 1 && !cluster_k) || balanced) {
         if (!transposed && v.N % 4) return fail(B200_GEMM_ERR_BAD_CONFIG, "split_k needs N %% 4 == 0 in the kernel view");
         if (fixed) {
@@ -1295,7 +1302,8 @@ static int launch_gemm(const Problem& p, cudaStream_t stream, const b200_gemm_co
                 CUDA_TRY(cudaMallocAsync(reinterpret_cast<void**>(&ws), ws_bytes, stream));
                 ws_stream_ordered = true;
             } else {
-                st = get_workspace(env.ctx, stream, ws_bytes, &ws);
+                ws_lock = env.ctx->lock_stream(stream);
+                st      = get_workspace(env.ctx, stream, ws_bytes, &ws);
                 if (st != B200_GEMM_OK) return st;
             }
         }

@@ -725,6 +725,40 @@ def test_two_host_threads(L):
         _grad_check(s)
 
 
+def test_two_host_threads_on_one_stream(L):
+    """Scratch of different sizes, growing, with K partitions and without: the calls' launches do not mix."""
+    import threading
+    gen = make_gen("one stream")
+    sets = [[_work_set(gen, M=m, N=n, K=k) for m, n, k in sizes] for sizes in
+            ([(700, 1032, 264), (300, 1000, 2056), (3001, 2056, 136)], [(1100, 520, 136), (333, 1000, 2056), (2500, 4104, 72)])]
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(mine):
+        try:
+            with torch.cuda.stream(st):
+                for i in range(60):
+                    for s in mine[:1 + i // 20]:
+                        _grad_call(L, s)
+                        L.gemm(s["p"], s["a"], s["b"], s["M"], s["N"], s["K"], layout_b=1)
+        except Exception as e:  # noqa: BLE001 (reported below)
+            errors.append(e)
+
+    for s in sets[0] + sets[1]:
+        s["p"] = torch.empty(s["M"], s["N"], device="cuda", dtype=torch.bfloat16)
+    threads = [threading.Thread(target=work, args=(m,)) for m in sets]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for s in sets[0] + sets[1]:
+        _grad_check(s)
+        check(s["p"], *product(s["a"], s["b"].t()))
+
+
 def test_results_repeat_bit_for_bit(L):
     gen = make_gen("repeat")
     s = _work_set(gen, M=2000, N=520, K=1032)
