@@ -269,6 +269,25 @@ class loader:
                                         int(layout_c), int(layout_a), int(layout_b)))
 
     # ---- products with epilogues, grouped products, gradients ------------------------------
+    def _types_of(self, C, A, types) -> int:
+        """`_type_index` for calls that check their arguments: a pair without a kernel, and `types` that are
+        not those of the tensors given, are a ValueError."""
+        if types is None:
+            try:
+                return self._type_index(C, A, None)
+            except (KeyError, AttributeError):
+                raise ValueError(f"no product {getattr(C, 'dtype', 'of an address')} from {getattr(A, 'dtype', 'an address')}: "
+                                 f"one of {', '.join(map(str, TYPE_PAIRS))} (addresses need types)") from None
+        pair = types if isinstance(types, tuple) else next((k for k, v in TYPE_PAIRS.items() if v == types), None)
+        if pair not in TYPE_PAIRS:
+            raise ValueError(f"unknown types {types!r}: one of {', '.join(map(str, TYPE_PAIRS))}")
+        for t, name in zip((C, A), pair):
+            if t is not None and not isinstance(t, int) and t.dtype != self._torch_type(t, self._TORCH_NAMES[name]):
+                raise ValueError(f"types {types!r} do not go with a {t.dtype} tensor")
+        return TYPE_PAIRS[pair]
+
+    _TORCH_NAMES = {"f16": "float16", "bf16": "bfloat16", "f32": "float32"}
+
     def _arguments(self, stream, spec):
         """(device to make current or None, stream cell, addresses) of a call's array arguments.
 
@@ -354,7 +373,7 @@ class loader:
         residual and preact C's layout; residual (forward) or preact (gradient) may be C itself.
         With batch_count > 1, `bias_stride` 0 shares one bias among the items (its gradient is
         the sum over them), N or more gives each its own."""
-        t = self._type_index(C, A, types)
+        t = self._types_of(C, A, types)
         mn, vec = batch_count * M * N, N + (batch_count - 1) * bias_stride if N else 0
         ct, it = getattr(C, "dtype", None), getattr(A, "dtype", None)
         dev, sp, (c, a, b, bi, re, pr, bg) = self._arguments(stream, (
@@ -372,7 +391,7 @@ class loader:
         int32 tensor of groups + 1 on the device; rows outside [offsets[0], offsets[groups]) are
         left as they are.  bias and bias_grad are groups x N.  The input gradient is the same call
         on the output's gradient with layout_b flipped and N and K exchanged."""
-        t = self._type_index(C, A, types)
+        t = self._types_of(C, A, types)
         mn, ct, it = rows * N, getattr(C, "dtype", None), getattr(A, "dtype", None)
         dev, sp, (c, a, b, bi, re, pr, bg, off) = self._arguments(stream, (
             ("C", C, mn, None), ("A", A, rows * K, None), ("B", B, groups * K * N, it),
@@ -388,7 +407,7 @@ class loader:
         """`b200_gemm_grouped_wgrad`: for every group `C_e = A[rows of e]^T * B[rows of e]` (added to
         C_e with `accumulate`), A rows x M, B rows x N, C groups x M x N, each C_e in layout_c.
         An empty group's C_e is zero."""
-        t = self._type_index(C, A, types)
+        t = self._types_of(C, A, types)
         dev, sp, (c, a, b, off) = self._arguments(stream, (
             ("C", C, groups * M * N, None), ("A", A, rows * M, None), ("B", B, rows * N, getattr(A, "dtype", None)),
             ("offsets", offsets, groups + 1, self._torch_type(offsets, "int32"))))
@@ -407,9 +426,11 @@ class loader:
             if loader._OUT_TYPES is None:
                 import torch
                 loader._OUT_TYPES = {torch.float16: 0, torch.float32: 3, torch.bfloat16: 2}
-            t = loader._OUT_TYPES[dY.dtype]
+            t = loader._OUT_TYPES.get(getattr(dY, "dtype", None))
+            if t is None:
+                raise ValueError(f"dY is {getattr(dY, 'dtype', 'an address')}: a float16, bfloat16 or float32 tensor, or give types")
         else:
-            t = TYPE_PAIRS[types] if isinstance(types, tuple) else int(types)
+            t = self._types_of(dY, None, types)
         mn, ct = batch_count * M * N, getattr(dY, "dtype", None)
         vec = groups * N if groups else (N + (batch_count - 1) * bias_stride if N else 0)
         dev, sp, (dz, dy, z, bg, off) = self._arguments(stream, (

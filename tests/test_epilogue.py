@@ -141,6 +141,31 @@ def test_python_names(gl):
         L.gemm_fused(C, A, B, 8, 8, 8, activation="gelu", gradient=True, types=2)
 
 
+@pytest.mark.parametrize("stride", (2 ** 64 - 64, 2 ** 63, 2 ** 48))
+def test_bias_strides_past_every_address(gl, stride):
+    """Refused: a stride that wraps (a negative one, say) must not pass for a vector inside the tensor."""
+    assert fused(gl, batch=3, bias=BIAS, bias_stride=stride) == BAD_SIZE
+    assert fused(gl, batch=3, gradient=1, bias_grad=BG, bias_stride=stride) == BAD_SIZE
+    assert backward(gl, batch=3, stride=stride) == BAD_SIZE
+
+
+def test_python_types(gl):
+    """Given types that are not the tensors', and pairs without a kernel."""
+    import torch
+    L = gl[0].loader()
+    t = {n: torch.zeros(64, dtype=getattr(torch, n)) for n in ("float16", "bfloat16", "float32", "float64")}
+    bf, f16, f32, f64 = t["bfloat16"], t["float16"], t["float32"], t["float64"]
+    for c, a, types in [(bf, bf, 3), (bf, bf, ("f32", "bf16")), (f32, bf, ("f32", "f16")), (C, bf, 1), (f32, B, 2), (bf, bf, 4),
+                        (bf, bf, ("bf16", "f16")), (bf, f16, None), (f64, f64, None), (f32, f32, None), (C, bf, None), (C, A, None)]:
+        for call in (lambda: L.gemm_fused(c, a, a, 8, 8, 8, types=types), lambda: L.gemm_grouped(c, a, a, OFF, 8, 8, 8, 1, types=types),
+                     lambda: L.gemm_grouped_wgrad(c, a, a, OFF, 8, 8, 8, 1, types=types)):
+            with pytest.raises(ValueError, match="types|product"):
+                call()
+    for dy, types in [(f64, None), (A, None), (bf, 3), (f32, ("f16", "f16")), (bf, 9)]:
+        with pytest.raises(ValueError, match="types"):
+            L.activation_backward(None, dy, PRE, 8, 8, activation="relu", types=types)
+
+
 CPP = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp")
 
 
