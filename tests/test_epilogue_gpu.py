@@ -808,3 +808,93 @@ def test_same_sizes_in_turn(L):
     for step in (1, 59, 101):  # (each without a common factor with the number of cases)
         for i in range(len(cases)):
             fused(L, 128, 256, 1024, **cases[i * step % len(cases)])
+
+
+# ------------------------------------------------------------------------------ corners of what the documentation allows
+def strided_bias(L, M, N, K, batch, stride, pair=("bf16", "bf16"), layouts=(0, 0, 1), act="silu"):
+    """Bias and bias gradient vectors further apart than they are long; what lies between is left as it is."""
+    out, dt = DTYPES[pair[0]], DTYPES[pair[1]]
+    lc, la, lb = layouts
+    gen = make_gen("stride", M, N, K, batch, stride)
+    a = randn(gen, batch, *((K, M) if la else (M, K)), dtype=dt)
+    b = randn(gen, batch, *((N, K) if lb else (K, N)), dtype=dt, scale=max(K, 1) ** -0.5)
+    A, B = view(a, M, K, la, (batch,)), view(b, K, N, lb, (batch,))
+    shape = (batch, N, M) if lc else (batch, M, N)
+    length = (batch - 1) * stride + N
+    where = (torch.arange(batch, device="cuda")[:, None] * stride + torch.arange(N, device="cuda")).flatten()
+    flat = torch.full((length,), float("nan"), dtype=out, device="cuda")
+    bias = randn(gen, batch, N, dtype=out)
+    flat[where] = bias.flatten()
+    c, z = Guarded(shape, out), Guarded(shape, out)
+    kw = dict(layout_c=lc, layout_a=la, layout_b=lb, batch_count=batch, activation=act, bias_stride=stride)
+    L.gemm_fused(c.t, a, b, M, N, K, bias=flat, preact=z.t, **kw)
+    y, ey, Z, ez = forward(A, B, act, bias[:, None, :])
+    check(view(c.t, M, N, lc, (batch,)), y, ey, "C")
+    check(view(z.t, M, N, lc, (batch,)), Z, ez, "preact")
+    sums = [Guarded((length,), torch.float32) for _ in range(2)]
+    for s in sums:
+        s.t.fill_(7.0)
+    Z = view(z.t, M, N, lc, (batch,)).clone()
+    L.gemm_fused(c.t, a, b, M, N, K, preact=z.t, gradient=True, bias_grad=sums[0].t, **kw)
+    d, ed = gradient(*product(A, B), Z, act)
+    check(view(c.t, M, N, lc, (batch,)), d, ed, "gradient")
+    dy = c.t.clone()
+    L.activation_backward(c.t, dy, z.t, M, N, layout=lc, batch_count=batch, activation=act, bias_grad=sums[1].t, bias_stride=stride)
+    d2, ed2 = gradient(view(dy, M, N, lc, (batch,)).double(), torch.zeros_like(d), Z, act)
+    check(view(c.t, M, N, lc, (batch,)), d2, ed2, "backward")
+    for s, (v, e) in zip(sums, ((d, ed), (d2, ed2))):
+        check_sum(s.t[where].view(batch, N), v, e, 1, "bias_grad")
+        s.t[where] = 7.0
+        assert (s.t == 7.0).all() and s.intact(), "wrote between the vectors"
+    assert c.intact() and z.intact()
+
+
+@pytest.mark.parametrize("layouts", [(0, 0, 1), (1, 0, 0)], ids=("rows", "columns"))
+@pytest.mark.parametrize("M,N,K,batch,stride", [(16, 136, 64, 3, 139), (160, 72, 136, 4, 1000), (192, 512, 8192, 2, 515), (16, 64, 2048, 5, 64), (9, 21, 13, 2, 22)])
+def test_fused_bias_stride(L, M, N, K, batch, stride, layouts):
+    strided_bias(L, M, N, K, batch, stride, layouts=layouts)
+    strided_bias(L, M, N, K, batch, stride, ("f32", "f16"), layouts, act="gelu")
+
+
+@pytest.mark.parametrize("layout_c", (0, 1))
+def test_many_items(L, layout_c):
+    """More batch items than a grid's second and third extent."""
+    for M, N, K, batch in [(3, 8, 8, 66000), (8, 5, 3, 70001)]:
+        fused(L, M, N, K, batch=batch, layouts=(layout_c, 0, 0), own_bias=True)
+        fused(L, M, N, K, batch=batch, layouts=(layout_c, 0, 0), own_bias=True, grad=True)
+        fused(L, M, N, K, batch=batch, layouts=(layout_c, 0, 0), grad=True)
+    strided_bias(L, 2, 8, 8, 66001, 9, layouts=(layout_c, 0, 0))
+
+
+@pytest.mark.parametrize("lb", (0, 1))
+def test_grouped_without_k_and_narrow(L, lb):
+    for N, K in [(136, 0), (1, 64), (8, 1), (1, 1), (5, 0)]:
+        for counts in (COUNTS["ragged"], COUNTS["all empty"], [700, 0, 500]):
+            grouped(L, counts, N, K, lb=lb, head=2, tail=3)
+            grouped(L, counts, N, K, ("f32", "f16"), lb=lb, grad=True, act="gelu_tanh", head=1)
+    for M, N in [(1, 1), (1, 264), (264, 1)]:
+        wgrad(L, COUNTS["ragged"], M, N, lc=lb)
+        wgrad(L, COUNTS["all empty"], M, N, lc=lb, accumulate=True)
+
+
+def test_no_rows_at_all(L):
+    """Every group empty and no rows: sums and weight gradients are zero, everything else is left alone."""
+    E, N, K = g.MAX_GROUPS, 24, 16
+    offs = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    bf = torch.bfloat16
+    none, w = torch.empty(0, K, device="cuda", dtype=bf), torch.ones(E, K, N, device="cuda", dtype=bf)
+    for call in ("product", "backward"):
+        bg = Guarded((E, N), torch.float32)
+        empty = torch.empty(0, N, device="cuda", dtype=bf)
+        if call == "product":
+            L.gemm_grouped(empty, none, w, offs, 0, N, K, E, activation="relu", preact=empty, gradient=True, bias_grad=bg.t)
+        else:
+            L.activation_backward(empty, empty, empty, 0, N, activation="relu", bias_grad=bg.t, offsets=offs, groups=E)
+        assert (bg.t == 0).all() and bg.intact()
+    dw = Guarded((E, K, N), torch.float32)
+    empty = torch.empty(0, N, device="cuda", dtype=bf)
+    L.gemm_grouped_wgrad(dw.t, none, empty, offs, 0, K, N, E)
+    assert (dw.t == 0).all()
+    dw.t.fill_(3.0)
+    L.gemm_grouped_wgrad(dw.t, none, empty, offs, 0, K, N, E, accumulate=True)
+    assert (dw.t == 3).all() and dw.intact()
