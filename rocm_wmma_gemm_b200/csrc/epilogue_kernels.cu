@@ -76,6 +76,7 @@ cudaError_t set_epilogue_attributes()
     if (e == cudaSuccess) e = set_one<256, 1, false, false>();
     if (e == cudaSuccess) e = set_one<256, 2, false, false>();
     if (e == cudaSuccess) e = set_one<512, 2, false, false>();
+    if (e == cudaSuccess) e = set_one<256, 2, true, false>();
     if (e == cudaSuccess) e = set_one<16, 1, true, false>();
     if (e == cudaSuccess) e = set_one<32, 1, true, false>();
     if (e == cudaSuccess) e = set_one<64, 1, true, false>();
@@ -90,7 +91,9 @@ cudaError_t set_epilogue_attributes()
 cudaError_t launch_epilogue_gemm(const EpilogueLaunch& l, cudaStream_t s)
 {
     const bool ks = l.split > 1;
-    if (l.tr) {
+    if (l.tr && l.cl == 2) {
+        if (l.bn == 256) return launch_one<256, 2, true, false>(l, s);
+    } else if (l.tr) {
         switch (l.bn) {
             case 16: return ks ? launch_one<16, 1, true, true>(l, s) : launch_one<16, 1, true, false>(l, s);
             case 32: return ks ? launch_one<32, 1, true, true>(l, s) : launch_one<32, 1, true, false>(l, s);

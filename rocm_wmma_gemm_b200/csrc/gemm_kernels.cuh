@@ -240,6 +240,7 @@ struct WorkCoord {
     uint32_t k_first;  // ragged K: first row of the group (0 otherwise)
     uint32_t end;      // end of the ragged extent's group: rows (columns with the transposed epilogue) from here on are not ours
     uint32_t group, first; // group, its first row
+    uint32_t wn;       // balanced ragged tiles: the tile's width
 };
 
 // Tile index -> (tile-row, tile-column) under the problem's raster.
@@ -435,7 +436,10 @@ __device__ __forceinline__ void tile_coords_epilogue(const GemmParams& p, const 
     m_idx = first_m + m_in;
 }
 
-template <bool TR>
+//
+// BALANCED (ragged rows along N, see the pair kernel with the transposing epilogue): a group's tiles are
+// equally wide, multiples of 32 columns, instead of bn wide with a narrow last one.
+template <bool TR, bool BALANCED = false>
 __device__ __forceinline__ bool work_next_epilogue(const GemmParams& p, const EpilogueParams& ep, const GroupTable& gt,
                                                    WorkCursor& cur, uint32_t units, int bn, int bm, WorkCoord& c)
 {
@@ -480,7 +484,9 @@ __device__ __forceinline__ bool work_next_epilogue(const GemmParams& p, const Ep
     c.group              = lo;
     c.first              = gt.first[lo];
     c.end                = gt.first[lo + 1u];
-    const uint32_t along = c.first + (in_g - o * rt) * static_cast<uint32_t>(TR ? bn : bm);
+    // (rt tiles of at most bn columns: the last one begins before the group ends whatever their width)
+    c.wn                 = BALANCED ? ((c.end - c.first + rt - 1u) / rt + 31u) & ~31u : static_cast<uint32_t>(TR ? bn : bm);
+    const uint32_t along = c.first + (in_g - o * rt) * c.wn;
     c.m0                 = TR ? o * static_cast<uint32_t>(bm) : along;
     c.n0                 = TR ? along : o * static_cast<uint32_t>(bn);
     c.z_a                = TR ? lo : 0u;
@@ -593,6 +599,14 @@ __device__ __forceinline__ uint32_t pack2(uint32_t lo_bits, uint32_t hi_bits)
 // loops.  The matrix an epilogue reads (residual, or Z in gradient mode) comes by TMA into the
 // staging buffer its chunk will leave from, requested before the accumulator is awaited, so its
 // latency hides under the main loop; Z leaves through a staging buffer of its own.
+//
+// EP && TR && CL == 2 (TRP): grouped products with more than a few rows per group.  The groups' matrices are
+// A' (256 of C's columns per tile and pair), C's rows are the MMA's N, which comes in steps of 32: a
+// group's rows are rounded up to 32 per tile, not to 256 as they would be along M (512 rows per
+// group on average: 25 % more products than asked for).  A group's tiles are equally wide; the MMA's N
+// extent is set per tile, and the box of rows is always 128 per CTA (boxes of just the rows wanted cost
+// more producer instructions than they save traffic: 16384 rows in 32 groups x 2048 x 4096 272 us in
+// boxes of 32, 256 in boxes of 64, 251 whole; 278 with the rows along M).
 // ---------------------------------------------------------------------------------------------
 // Maps of the matrices beside C: the one the epilogue reads, and where Z goes.
 struct EpilogueMaps {
@@ -1136,6 +1150,141 @@ struct EpilogueColumns {
     }
 };
 
+// One epilogue warp of the pair kernel with the transposing epilogue: chunks of 32 columns (of C's rows)
+// from col0 on by the 32 kernel rows from row0 on (one per lane; contiguous in C), staged as 32 lines
+// of 32 elements (no swizzle: a warp's accesses are whole lines), which TMA moves from and to C and the
+// matrices like it.  A bias is one value per lane, its gradient a sum over a lane's registers.  Ragged
+// rows only.
+template <int OUT>
+struct EpilogueTransposed {
+    using T = OutType<OUT>;
+    static constexpr uint32_t LINE = 32u * sizeof(T), BUF = 32u * LINE;
+
+    const GemmParams&     p;
+    const EpilogueParams& ep;
+    const EpilogueMaps&   em;
+    const CUtensorMap&    tmD;
+    uint32_t              lane;
+    uint32_t              stg;    // staging buffers: ep.bufs for C, then one for Z
+    uint32_t              in_bar; // barriers of the first two
+    volatile uint32_t*    s_abort;
+    uint32_t              count     = 0; // as in EpilogueWarp
+    uint32_t              in_phase  = 0;
+    uint32_t              in_flight = 0;
+
+    __device__ __forceinline__ uint32_t slot(uint32_t k) const { return (count + k) & (ep.bufs - 1u); }
+
+    __device__ __forceinline__ void request(uint32_t k, uint32_t row0, uint32_t col0)
+    {
+        const uint32_t b = slot(k);
+        if (lane == 0) {
+            ptx::mbar_expect_tx(in_bar + 8u * b, BUF);
+            ptx::tma_load_3d(stg + b * BUF, &em.in, in_bar + 8u * b, row0, col0, 0, 0);
+        }
+        in_flight |= 1u << b;
+    }
+
+    __device__ __forceinline__ void buffers_free()
+    {
+        ptx::fence_proxy_async_smem();
+        if (lane == 0) ptx::tma_store_wait_read<0>();
+        __syncwarp();
+    }
+
+    __device__ __forceinline__ float row_bias(const WorkCoord& c, uint32_t row) const
+    {
+        if (!ep.bias || row >= p.M) return 0.f;
+        return to_f32(static_cast<const T*>(ep.bias)[c.group * ep.bias_stride + row]);
+    }
+
+    // Columns [col0, min(col0 + 32, stop)) are the group's.  False: a wait ran out.
+    template <class F>
+    __device__ __forceinline__ bool chunk(const WorkCoord& c, uint32_t row0, uint32_t col0, uint32_t stop, float bias, TmemPieces<COLUMN_PIECE>& pieces, F&& accumulators_read)
+    {
+        const uint32_t b    = slot(0);
+        const uint32_t sbuf = stg + b * BUF, xbuf = stg + ep.bufs * BUF, at = lane * static_cast<uint32_t>(sizeof(T));
+        if (ep.streamed) {
+            bool ok = bounded_wait(in_bar + 8u * b, (in_phase >> b) & 1u, s_abort, p.status, ST_EPI_WAIT);
+            ok      = __all_sync(0xffffffffu, ok);
+            if (!ok) return false;
+            in_phase ^= 1u << b;
+            in_flight &= ~(1u << b);
+        }
+        // the buffers written below must have been read by the stores that last used them
+        if (lane == 0) {
+            if (ep.aux || ep.bufs == 1u) ptx::tma_store_wait_read<0>();
+            else if (!ep.streamed) ptx::tma_store_wait_read<1>();
+        }
+        __syncwarp();
+        float row_sum = 0.f;
+#pragma unroll 1
+        for (uint32_t pc = 0; pc < 32u / COLUMN_PIECE; ++pc) {
+            const uint32_t first = pc * COLUMN_PIECE, to = sbuf + first * LINE + at;
+            float          v[COLUMN_PIECE], side[COLUMN_PIECE];
+            pieces.get(pc, v, accumulators_read);
+            if (ep.streamed)
+#pragma unroll
+                for (uint32_t j = 0; j < COLUMN_PIECE; ++j) side[j] = to_f32(ld_shared_elem<T>(to + j * LINE));
+            if (ep.gradient) {
+                if (ep.streamed) apply_slope(ep, v, side);
+            } else {
+                if (ep.bias)
+#pragma unroll
+                    for (uint32_t j = 0; j < COLUMN_PIECE; ++j) v[j] += bias;
+                if (ep.aux)
+#pragma unroll
+                    for (uint32_t j = 0; j < COLUMN_PIECE; ++j) st_shared_elem(xbuf + (first + j) * LINE + at, from_f32<T>(v[j]));
+                apply_activation(ep, v);
+                if (ep.streamed) add_values(v, side);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < COLUMN_PIECE; ++j) st_shared_elem(to + j * LINE, from_f32<T>(v[j]));
+            if (ep.part)
+#pragma unroll
+                for (uint32_t j = 0; j < COLUMN_PIECE; ++j) row_sum += col0 + first + j < stop ? v[j] : 0.f;
+        }
+        const uint32_t row = row0 + lane;
+        if (ep.part && row < p.M)
+            ep.part[(static_cast<uint64_t>(group_first_block(c.first, c.group, 32u)) + (col0 - c.first) / 32u) * p.M + row] = row_sum;
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (col0 + 32u <= stop) {
+            if (lane == 0) {
+                ptx::tma_store_3d(&tmD, sbuf, row0, col0, 0, 0);
+                if (ep.aux) ptx::tma_store_3d(&em.aux, xbuf, row0, col0, 0, 0);
+            }
+        } else if (row < p.M) { // the lines from `stop` on are the next group's
+            const uint64_t to = static_cast<uint64_t>(col0) * p.M + row;
+            for (uint32_t j = 0; j < stop - col0; ++j) {
+                static_cast<T*>(p.out)[to + static_cast<uint64_t>(j) * p.M] = ld_shared_elem<T>(sbuf + j * LINE + at);
+                if (ep.aux) static_cast<T*>(ep.preact)[to + static_cast<uint64_t>(j) * p.M] = ld_shared_elem<T>(xbuf + j * LINE + at);
+            }
+        }
+        if (lane == 0) ptx::tma_store_commit(); // (an empty group keeps the count of the waits)
+        __syncwarp();
+        ++count;
+        return true;
+    }
+
+    // After a give-up: the loads still in flight must land before this CTA's memory goes away.
+    __device__ __forceinline__ void drain()
+    {
+        if (lane == 0) {
+            for (uint32_t b = 0; b < 2u; ++b) {
+                if (!((in_flight >> b) & 1u)) continue;
+                const uint64_t t0 = ptx::global_timer_ns();
+                while (!ptx::mbar_try_wait(in_bar + 8u * b, (in_phase >> b) & 1u)) {
+                    if (ptx::global_timer_ns() - t0 > WAIT_LIMIT_NS) {
+                        atomicOr(p.status, ST_DRAIN_WAIT);
+                        break;
+                    }
+                }
+            }
+            ptx::tma_store_wait_read<0>();
+        }
+    }
+};
+
 template <int BN, int OUT, int CL, bool TR, bool GATHER, bool KS = false, bool EP = false>
 __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUtensorMap& tmB,
                                                const CUtensorMap* tmDs, const CUtensorMap& tmW, const GemmParams& p,
@@ -1145,7 +1294,8 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
     static_assert(BN == 16 || BN == 32 || BN == 64 || BN == 128 || BN == 256 || BN == 512,
                   "BN must be 16, 32, 64, 128, 256 or 512");
     static_assert(CL == 1 || CL == 2, "cluster size must be 1 or 2");
-    static_assert(!TR || CL == 1, "the transposed epilogue is a one-CTA variant");
+    static_assert(!TR || CL == 1 || (EP && BN == 256), "the transposed epilogue: one-CTA kernels, and the pair kernel of ragged rows");
+    constexpr bool TRP = TR && CL == 2; // ragged rows along N, tiles of equal width per group, a staged transposing epilogue
     static_assert(!KS || (CL == 1 && !GATHER && ((!TR && BN >= 128 && BN <= 256) || (TR && BN <= 128))),
                   "cluster K partitions: one-CTA staged tiles of 128 or 256 columns, transposed slabs of up to 128");
     // One MMA covers at most 256 columns: a 512-wide tile is two sub-tiles that share the A'
@@ -1189,7 +1339,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
     static_assert(!EP || !GATHER, "no gathering kernels with an epilogue");
     constexpr int                    EPW = EP ? EPI_WARPS : 4; // epilogue warps
     __shared__ volatile uint32_t     s_seen[2];                                          // EP: the accumulator awaited last is complete
-    __shared__ __align__(8) uint64_t s_in[EP && !TR ? EPI_WARPS * 2 : 1];                // EP: chunk of the read matrix landed
+    __shared__ __align__(8) uint64_t s_in[EP && (!TR || CL == 2) ? EPI_WARPS * 2 : 1];                // EP: chunk of the read matrix landed
     constexpr uint32_t               BIAS_BYTES = (UMMA_N < 32 * EPI_WARPS ? 32 * EPI_WARPS : UMMA_N) * OUT_BYTES;
     __shared__ __align__(16) uint8_t s_bias[EP && !TR ? 2 * BIAS_BYTES : 16];            // EP: a tile's biases, two tiles in turn
 
@@ -1241,7 +1391,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
         }
     }
     auto next_work = [&](WorkCursor& cur, WorkCoord& c) -> bool {
-        if constexpr (EP) return work_next_epilogue<TR>(p, *epp, gt, cur, units, wn, tile_m, c);
+        if constexpr (EP) return work_next_epilogue<TR, TRP>(p, *epp, gt, cur, units, wn, tile_m, c);
         else return work_next(p, cur, unit, units, wn, tile_m, c);
     };
 
@@ -1267,7 +1417,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             ptx::mbar_init(ptx::smem_u32(&s_tfull[lane - 30u]), 1);
             ptx::mbar_init(ptx::smem_u32(&s_tempty[lane - 30u]), EPW * CL);
         }
-        if constexpr (EP && !TR) {
+        if constexpr (EP && (!TR || TRP)) {
             if (lane < EPI_WARPS * 2) ptx::mbar_init(ptx::smem_u32(&s_in[lane]), 1);
         }
         ptx::fence_mbar_init();
@@ -1330,7 +1480,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                     c.k_first = 0u;
                 }
                 const int32_t   am = static_cast<int32_t>(c.m0 + rank * BLOCK_M);
-                const int32_t   bn = static_cast<int32_t>(c.n0 + rank * sub_rows);
+                const int32_t   bn = static_cast<int32_t>(c.n0 + rank * (TRP ? c.wn / 2u : sub_rows));
                 // Streaming (HBM-bound) problems rotate each work unit's K order so that the CTAs
                 // running at the same time read different K offsets: rows of a K-major operand
                 // are a power of two apart, and same-offset reads from thousands of rows land on
@@ -1583,6 +1733,8 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         }
                     }
                 } else {
+                    // (bits 17 .. 22: the MMA's N extent / 8)
+                    const uint32_t idesc = TRP ? (p.idesc & ~(0x3fu << 17)) | ((c.wn >> 3) << 17) : p.idesc;
                     for (uint32_t kb = c.kb0; kb < c.kb1; ++kb) {
                         ok = bounded_wait(ptx::smem_u32(&s_full[stage]), phase, &s_abort, p.status,
                                           ST_MMA_WAIT_FULL);
@@ -1595,7 +1747,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         const uint64_t bd = ptx::make_smem_desc(sb, b_lbo, 1024u);
 #pragma unroll
                         for (uint32_t k = 0; k < BLOCK_K / UMMA_K; ++k) {
-                            ptx::umma_f16<CL>(d_tmem, ad + k * a_kstep, bd + k * b_kstep, p.idesc,
+                            ptx::umma_f16<CL>(d_tmem, ad + k * a_kstep, bd + k * b_kstep, idesc,
                                               (kb > c.kb0 || k > 0u) ? 1u : 0u);
                         }
                         // Slot free (in both CTAs of a pair) once these MMAs retire.
@@ -1670,6 +1822,43 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                 ks_c  = c;
                 ks_ok = ok;
             }
+        } else if constexpr (TRP) {
+            using ET = EpilogueTransposed<OUT>;
+            ET   et{p, *epp, *em, tmD, lane, epi + (warp - 2u) * (epp->bufs + epp->aux) * ET::BUF, ptx::smem_u32(&s_in[(warp - 2u) * 2u]), &s_abort};
+            bool live_warp = true;
+            for (; ok && next_work(cur, c); ++it) {
+                const uint32_t buf  = it % NUM_ACC;
+                const uint32_t row0 = c.m0 + rank * BLOCK_M + q * 32u;
+                const uint32_t stop = min(c.end, c.n0 + c.wn);
+                const uint32_t live = row0 < p.M && c.n0 < stop ? (stop - c.n0 + 31u) / 32u : 0u;
+                const uint32_t mine = live > hw ? (live - hw + EPI_SETS - 1u) / EPI_SETS : 0u; // this warp's chunks: hw, hw + EPI_SETS, ...
+                auto           col  = [&](uint32_t k) { return c.n0 + (hw + EPI_SETS * k) * 32u; };
+                const uint32_t tacc = tmem_base + ((q * 32u) << 16) + buf * ACC_COLS;
+                float          bias = 0.f;
+                if (mine && live_warp) {
+                    dep_wait();
+                    if (epp->streamed) {
+                        et.buffers_free();
+                        for (uint32_t k = 0; k < min(epp->bufs, mine); ++k) et.request(k, row0, col(k));
+                    }
+                    bias = et.row_bias(c, row0 + lane);
+                }
+                ok = accumulator(buf, (it / NUM_ACC) & 1u);
+                if (!ok) break;
+                if (!live_warp) continue; // (it still meets the others at every accumulator)
+                if (mine == 0u) release(buf);
+#pragma unroll 1
+                for (uint32_t k = 0; k < mine; ++k) {
+                    TmemPieces<COLUMN_PIECE> pieces{tacc + (hw + EPI_SETS * k) * 32u, 32u / COLUMN_PIECE, c.kb1 == c.kb0};
+                    if (epp->streamed && k > 0u && k - 1u + epp->bufs < mine) {
+                        et.buffers_free(); // the chunk before this one left from the buffer asked for now
+                        et.request(epp->bufs - 1u, row0, col(k - 1u + epp->bufs));
+                    }
+                    live_warp = et.chunk(c, row0, col(k), stop, bias, pieces, [&] { if (k + 1u == mine) release(buf); });
+                    if (!live_warp) break; // (a wait ran out: the abort flag ends the other roles)
+                }
+            }
+            et.drain();
         } else if constexpr (TR) {
             const EpilogueColumns<OUT> ec{p, *epp, lane};
             constexpr uint32_t         CHUNKS = (BN + 31) / 32;

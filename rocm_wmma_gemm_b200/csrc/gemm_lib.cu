@@ -640,7 +640,8 @@ static void adapt_config(b200_gemm_config& c, const View& v, size_t batch, int s
 // TMA descriptors
 // ------------------------------------------------------------------------------------------
 static int encode_map(CUtensorMap* tm, CUtensorMapDataType dt, size_t esz, const void* base,
-                      uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b0, uint32_t b1, uint64_t pitch = 0)
+                      uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b0, uint32_t b1, uint64_t pitch = 0,
+                      CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B)
 {
     const cuuint64_t dims[3]    = {d0, d1, d2};
     const cuuint64_t line       = pitch ? pitch : d0; // elements from one line to the next
@@ -648,7 +649,7 @@ static int encode_map(CUtensorMap* tm, CUtensorMapDataType dt, size_t esz, const
     const cuuint32_t box[3]     = {b0, b1, 1};
     const cuuint32_t estr[3]    = {1, 1, 1};
     const CUresult   r = g_encode(tm, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
-                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return fail(B200_GEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) dims=%llu,%llu,%llu box=%u,%u", (int)r,
