@@ -58,6 +58,7 @@ struct EpilogueParams {
     uint32_t           aux;          // Z is written (EpilogueMaps::aux)
     uint32_t           unaligned;    // TMA cannot address C or the matrices like it
     uint32_t           plain;        // nothing but the conversion to C's type
+    uint32_t           whole_a, whole_b; // pairs: an MN-major operand's 128 rows arrive in one box (encode_operand_pair)
     uint32_t           bufs;         // staging buffers per warp for C: 1 or 2
     uint32_t           table_at;     // ragged: byte offset of the group table in dynamic shared memory
     FastDiv            per_item, per_band, per_column; // tiles per batch item (ragged rows: of the other extent), per raster band, rows per band or column

@@ -631,8 +631,7 @@ __device__ __forceinline__ float warp_column_sums(float (&v)[N], uint32_t lane)
     else return v[0];
 }
 
-// The epilogues work in pieces of 32 columns (16 where the accumulator is read transposed), in
-// loops that are not unrolled: the whole of a piece - bias, activation, residual, conversion - is a few
+// The epilogues work in pieces of 16 columns, in loops that are not unrolled: the whole of a piece - bias, activation, residual, conversion - is a few
 // hundred instructions, which stay in the instruction cache.
 constexpr int PIECE = 16, COLUMN_PIECE = 16;
 
@@ -1573,6 +1572,8 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                     }
                     if (p.a_mn_major == 0u) {
                         tma_load<CL>(sa, mapA, bar, k0, am, c.z_a, pol_a);
+                    } else if (EP && CL == 2 && epp->whole_a) {
+                        ptx::tma_load_4d_pair(sa, mapA, bar, 0, k0, am / 64, c.z_a);
                     } else {
 #pragma unroll
                         for (int j = 0; j < BLOCK_M / 64; ++j)
@@ -1586,6 +1587,8 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         const uint32_t sh = sb + h * SUB_BYTES;
                         if (p.b_mn_major == 0u) {
                             tma_load<CL>(sh, mapB, bar, k0, bh, c.z_b, pol_b);
+                        } else if (EP && CL == 2 && epp->whole_b) {
+                            ptx::tma_load_4d_pair(sh, mapB, bar, 0, k0, bh / 64, c.z_b);
                         } else {
 #pragma unroll
                             for (int j = 0; j < SUB_ROWS / 64; ++j)
