@@ -274,7 +274,7 @@ class loader:
         not those of the tensors given, are a ValueError."""
         if types is None:
             try:
-                return self._type_index(C, A, None)
+                return self._DTYPE_INDEX[C.dtype, A.dtype] if self._DTYPE_INDEX is not None else self._type_index(C, A, None)
             except (KeyError, AttributeError):
                 raise ValueError(f"no product {getattr(C, 'dtype', 'of an address')} from {getattr(A, 'dtype', 'an address')}: "
                                  f"one of {', '.join(map(str, TYPE_PAIRS))} (addresses need types)") from None
@@ -354,13 +354,18 @@ class loader:
             raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
         return act
 
+    _TORCH_TYPES = {}  # name -> torch's dtype, filled on first use
+
     @staticmethod
     def _torch_type(t, name):
         """torch's dtype `name` where t is a tensor (raw addresses need no torch)."""
         if t is None or isinstance(t, int):
             return None
-        import torch
-        return getattr(torch, name)
+        dtype = loader._TORCH_TYPES.get(name)
+        if dtype is None:
+            import torch
+            dtype = loader._TORCH_TYPES[name] = getattr(torch, name)
+        return dtype
 
     def gemm_fused(self, C, A, B, M, N, K, layout_c=0, layout_a=0, layout_b=0, batch_count=1, activation="none",
                    bias=None, residual=None, preact=None, gradient=False, bias_grad=None, bias_stride=0,
