@@ -43,7 +43,7 @@ struct EpilogueParams {
     float*         part;        // gradient: nullptr or partial bias gradients [batch][part_blocks][length]
     uint64_t       bias_stride; // elements between the biases of consecutive batch items / groups
     uint32_t       act;
-    float          k0, k1;      // ACT_SIGMOID: -c0 log2(e), -c1 log2(e)
+    float          k0, k1;      // ACT_SIGMOID: -c0 log2(e), -c1 log2(e); silu's k1 is the smallest normal number, so that k1 x^2 is not 0 times infinity
     float          slope0, slope1; // ACT_SIGMOID: c0, 3 c1
     uint32_t       gradient;
     uint32_t       part_blocks; // blocks per batch item (all groups together)
@@ -85,21 +85,61 @@ __device__ __forceinline__ float2 rcp(float2 x) { return make_float2(rcp(x.x), r
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// Minimum and maximum that keep a NaN.
+__device__ __forceinline__ float min_nan(float a, float b)
+{
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// Arguments are taken at most this large where an infinity would meet a factor that has become 0
+// (NaN): x itself, or x^2, which overflows from 1.8e19 on.  Every sigmoid and tail here is 0 or 1
+// in f32 from |x| = 105 on, so nothing else changes, and the infinities get the limits (a Z that has
+// overflowed in f16 has a slope).  Cost, 4096 x 4096 x 1024: value 33.5 -> 34.1 us, slope 46.6 -> 47.4
+// (silu and tanh gelu); nothing with the exact gelu, whose formulas are shorter in |x|.
+constexpr float FAR = 1e9f;
+__device__ __forceinline__ float2 not_below(float2 x) { return make_float2(max_nan(x.x, -FAR), max_nan(x.y, -FAR)); }
+__device__ __forceinline__ float2 not_above(float2 x) { return make_float2(min_nan(x.x, FAR), min_nan(x.y, FAR)); }
+
+// The same for pairs of 16-bit values (f16: the infinities become the largest values), where the slope is
+// a sigmoid's; half the instructions.
+template <uint32_t ACT, class T, int N>
+__device__ __forceinline__ void limit_words(uint32_t (&w)[N])
+{
+    if constexpr (ACT == ACT_SIGMOID && sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (std::is_same_v<T, __half>)
+                asm("max.NaN.f16x2 %0, %0, %1;\n\tmin.NaN.f16x2 %0, %0, %2;" : "+r"(w[i]) : "r"(0xfbfffbffu), "r"(0x7bff7bffu));
+            else
+                asm("max.NaN.bf16x2 %0, %0, %1;\n\tmin.NaN.bf16x2 %0, %0, %2;" : "+r"(w[i]) : "r"(0xce6ece6eu), "r"(0x4e6e4e6eu)); // FAR
+        }
+    }
+}
+
 // sigmoid(x (c0 + c1 x^2)) for k0 = -c0 log2(e), k1 = -c1 log2(e); x2 = x^2.  Far left 2^s overflows to
-// infinity and its reciprocal is 0, which is right.
+// infinity and its reciprocal is 0, which is right; so it is where x2 has overflowed.
 __device__ __forceinline__ float2 sigmoid_of(float2 x, float2 x2, float k0, float k1)
 {
     const float2 s = __fmul2_rn(x, __ffma2_rn(x2, splat(k1), splat(k0)));
     return rcp(__fadd2_rn(ex2(s), splat(1.f)));
 }
 
-// Normal distribution: tail = 1 - Phi(|x|) and e = exp(-x^2 / 2), which the density shares.  The tail is
-// e / 2 times a polynomial in t = 1 / (1 + 0.3275911 |x| / sqrt 2): Abramowitz and Stegun 7.1.26, erf
-// within 1.5e-7; in f32 the tail is within 3e-7.
-__device__ __forceinline__ void normal_tail(float2 x, float2 x2, float2& tail, float2& e)
+// Normal distribution for a = |x| <= FAR: tail = 1 - Phi(a) and e = exp(-a^2 / 2), which the density shares.
+// The tail is e / 2 times a polynomial in t = 1 / (1 + 0.3275911 a / sqrt 2): Abramowitz and Stegun 7.1.26,
+// erf within 1.5e-7; in f32 the tail is within 0.75e-7 + 5.5e-7 e.  The error is absolute: relative to
+// the tail it is 5e-5 at a = 3, 1.6e-3 at 5 and 3.6e-3 at 6.
+__device__ __forceinline__ void normal_tail(float2 a, float2& tail, float2& e)
 {
-    const float2 t = rcp(make_float2(fmaf(fabsf(x.x), 0.23164190f, 1.f), fmaf(fabsf(x.y), 0.23164190f, 1.f)));
-    e              = ex2(__fmul2_rn(x2, splat(-0.5f * LOG2E)));
+    const float2 t = rcp(__ffma2_rn(a, splat(0.23164190f), splat(1.f)));
+    e              = ex2(__fmul2_rn(__fmul2_rn(a, a), splat(-0.5f * LOG2E)));
     float2 q       = __ffma2_rn(t, splat(0.5f * 1.061405429f), splat(0.5f * -1.453152027f));
     q              = __ffma2_rn(q, t, splat(0.5f * 1.421413741f));
     q              = __ffma2_rn(q, t, splat(0.5f * -0.284496736f));
@@ -114,33 +154,39 @@ __device__ __forceinline__ float2 act_value(float2 x, const EpilogueParams& ep)
     if constexpr (ACT == ACT_RELU) {
         return make_float2(x.x < 0.f ? 0.f : x.x, x.y < 0.f ? 0.f : x.y);
     } else if constexpr (ACT == ACT_SIGMOID) {
-        return __fmul2_rn(x, sigmoid_of(x, __fmul2_rn(x, x), ep.k0, ep.k1));
+        const float2 c = not_below(x); // (only minus infinity would meet a 0)
+        return __fmul2_rn(c, sigmoid_of(c, __fmul2_rn(c, c), ep.k0, ep.k1));
     } else if constexpr (ACT == ACT_GELU) {
-        float2 tail, e;
-        normal_tail(x, __fmul2_rn(x, x), tail, e);
-        const float2 y = __fmul2_rn(x, tail); // x Phi(x) = x tail on the left, x - x tail on the right
-        return make_float2(x.x > 0.f ? x.x - y.x : y.x, x.y > 0.f ? x.y - y.y : y.y);
+        const float2 a = not_above(make_float2(fabsf(x.x), fabsf(x.y)));
+        float2       tail, e;
+        normal_tail(a, tail, e);
+        // x Phi(x) = -a tail on the left, x - a tail on the right (fmaxf loses a NaN, a keeps it)
+        return __ffma2_rn(make_float2(-a.x, -a.y), tail, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
     } else {
         return x;
     }
 }
 
-template <uint32_t ACT>
+// LIMITED: x has been through limit_words.
+template <uint32_t ACT, bool LIMITED = false>
 __device__ __forceinline__ float2 act_slope(float2 x, const EpilogueParams& ep)
 {
     if constexpr (ACT == ACT_RELU) {
         return make_float2(x.x > 0.f ? 1.f : (x.x <= 0.f ? 0.f : x.x), x.y > 0.f ? 1.f : (x.y <= 0.f ? 0.f : x.y));
     } else if constexpr (ACT == ACT_SIGMOID) {
         // d/dx x s(u(x)) = s + x s (1 - s) u'(x),  u = c0 x + c1 x^3
-        const float2 x2 = __fmul2_rn(x, x);
-        const float2 s  = sigmoid_of(x, x2, ep.k0, ep.k1);
-        const float2 w  = __fmul2_rn(__fmul2_rn(x, s), __ffma2_rn(s, splat(-1.f), splat(1.f)));
+        const float2 c  = LIMITED ? x : not_above(not_below(x));
+        const float2 x2 = __fmul2_rn(c, c);
+        const float2 s  = sigmoid_of(c, x2, ep.k0, ep.k1);
+        const float2 w  = __fmul2_rn(__fmul2_rn(c, s), __ffma2_rn(s, splat(-1.f), splat(1.f)));
         return __ffma2_rn(w, __ffma2_rn(x2, splat(ep.slope1), splat(ep.slope0)), s);
     } else if constexpr (ACT == ACT_GELU) {
-        float2 tail, e;
-        normal_tail(x, __fmul2_rn(x, x), tail, e);
-        const float2 phi = make_float2(x.x > 0.f ? 1.f - tail.x : tail.x, x.y > 0.f ? 1.f - tail.y : tail.y);
-        return __ffma2_rn(__fmul2_rn(x, splat(0.39894228f)), e, phi);
+        // Phi(x) + x phi(x) = r on the left and 1 - r on the right, r = tail(a) - a phi(a)
+        const float2 a = not_above(make_float2(fabsf(x.x), fabsf(x.y)));
+        float2       tail, e;
+        normal_tail(a, tail, e);
+        const float2 r = __ffma2_rn(__fmul2_rn(a, splat(-0.39894228f)), e, tail);
+        return make_float2(x.x > 0.f ? 1.f - r.x : r.x, x.y > 0.f ? 1.f - r.y : r.y);
     } else {
         return splat(1.f);
     }
@@ -439,7 +485,7 @@ struct ActBackwardParams {
 // V neighbouring elements: 16 bytes, or one.
 template <class T, int V>
 struct Pack {
-    T v[V];
+    alignas(V > 1 ? 16 : sizeof(T)) T v[V];
     __device__ __forceinline__ void load(const T* from)
     {
         if constexpr (V > 1) {
@@ -457,17 +503,35 @@ struct Pack {
     }
 };
 
+// Two neighbouring values as f32 and back, by the packed conversions.
+template <class T>
+__device__ __forceinline__ float2 load_pair(const T* from)
+{
+    if constexpr (sizeof(T) == 4) return make_float2(from[0], from[1]);
+    else if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(from));
+    else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(from));
+}
+template <class T>
+__device__ __forceinline__ void store_pair(T* to, float2 v)
+{
+    if constexpr (sizeof(T) == 4) to[0] = v.x, to[1] = v.y;
+    else if constexpr (std::is_same_v<T, __half>) *reinterpret_cast<__half2*>(to) = __float22half2_rn(v);
+    else *reinterpret_cast<__nv_bfloat162*>(to) = __float22bfloat162_rn(v);
+}
+
 // g becomes dZ = g act'(x); its f32 values are added to `sum`.
 template <uint32_t ACT, class T, int V>
-__device__ __forceinline__ void act_backward_pack(Pack<T, V>& g, const Pack<T, V>& x, float (&sum)[V], const EpilogueParams& ep)
+__device__ __forceinline__ void act_backward_pack(Pack<T, V>& g, Pack<T, V>& x, float (&sum)[V], const EpilogueParams& ep)
 {
     if constexpr (V > 1) {
+        if constexpr (sizeof(T) == 2) limit_words<ACT, T>(reinterpret_cast<uint32_t (&)[V / 2]>(x.v));
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
-            float2 v = make_float2(to_f32(g.v[i]), to_f32(g.v[i + 1]));
-            if constexpr (ACT != ACT_NONE) v = __fmul2_rn(v, act_slope<ACT>(make_float2(to_f32(x.v[i]), to_f32(x.v[i + 1])), ep));
-            g.v[i] = from_f32<T>(v.x), g.v[i + 1] = from_f32<T>(v.y);
-            sum[i] += v.x, sum[i + 1] += v.y;
+            float2 v = load_pair(g.v + i);
+            if constexpr (ACT != ACT_NONE) v = __fmul2_rn(v, act_slope<ACT, sizeof(T) == 2>(load_pair(x.v + i), ep));
+            store_pair(g.v + i, v);
+            const float2 t = __fadd2_rn(make_float2(sum[i], sum[i + 1]), v);
+            sum[i] = t.x, sum[i + 1] = t.y;
         }
     } else {
         float v = to_f32(g.v[0]);

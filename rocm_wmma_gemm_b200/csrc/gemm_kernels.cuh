@@ -761,6 +761,27 @@ __device__ __forceinline__ void unpack16(const uint32_t (&w)[4], float* v)
     }
 }
 
+// apply_slope for Z as it is stored: N values in 16-byte units.
+template <int OUT, int N, int UNITS>
+__device__ __forceinline__ void apply_slope(const EpilogueParams& ep, float (&v)[N], uint32_t (&w)[UNITS][4])
+{
+    with_act(ep.act, [&](auto tag) {
+        constexpr uint32_t ACT = decltype(tag)::value;
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            constexpr int UNIT = N / UNITS;
+            float         z[UNIT];
+            limit_words<ACT, OutType<OUT>>(w[i]);
+            unpack16<OUT>(w[i], z);
+#pragma unroll
+            for (int j = 0; j < UNIT; j += 2) {
+                const float2 y = __fmul2_rn(make_float2(v[i * UNIT + j], v[i * UNIT + j + 1]), act_slope<ACT, OUT != OUT_F32>(make_float2(z[j], z[j + 1]), ep));
+                v[i * UNIT + j] = y.x, v[i * UNIT + j + 1] = y.y;
+            }
+        }
+    });
+}
+
 template <int OUT>
 __device__ __forceinline__ void pack16(const float* v, uint32_t (&w)[4])
 {
@@ -971,14 +992,10 @@ struct EpilogueWarp {
             pieces.get(pc, v, accumulators_read);
             if (ep.gradient) {
                 if (ep.streamed) {
-                    float z[PIECE];
+                    uint32_t w[UNITS][4];
 #pragma unroll
-                    for (uint32_t i = 0; i < UNITS; ++i) {
-                        uint32_t w[4];
-                        ptx::ld_shared_v4(srow ^ (i << 4), w[0], w[1], w[2], w[3]);
-                        unpack16<OUT>(w, z + i * UNIT);
-                    }
-                    apply_slope(ep, v, z);
+                    for (uint32_t i = 0; i < UNITS; ++i) ptx::ld_shared_v4(srow ^ (i << 4), w[i][0], w[i][1], w[i][2], w[i][3]);
+                    apply_slope<OUT>(ep, v, w);
                 }
             } else {
                 if (col_bias) {
