@@ -310,22 +310,26 @@ class loader:
                 addresses.append(t.data_ptr())
         if device is None:
             return None, self._stream_ptr(stream), addresses
-        if loader._raw_stream is None:
-            import torch
-            loader._torch_cuda = torch.cuda
-            loader._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-                lambda index: torch.cuda.current_stream(index).cuda_stream)
-            loader._raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        raw_stream, raw_device, _ = loader._cuda or loader._cuda_calls()
         if stream is None:
-            handle = loader._raw_stream(device)
+            handle = raw_stream(device)
         else:
             owner = getattr(stream, "device_index", device)
             if owner != device:
                 raise ValueError(f"the stream is on device {owner}, the tensors on device {device}")
             handle = int(getattr(stream, "cuda_stream", stream))
-        return (device if loader._raw_device() != device else None), self._cell(handle), addresses
+        return (device if raw_device() != device else None), self._cell(handle), addresses
 
-    _raw_stream = _raw_device = _torch_cuda = None  # filled on the first call with tensors
+    _cuda = None  # (a device's current raw stream, the current device, torch.cuda), from the first call with tensors on
+
+    @staticmethod
+    def _cuda_calls():
+        import torch
+        stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
+        calls = (stream, getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device), torch.cuda)
+        loader._cuda = calls  # (in one piece: another thread finds all of it or nothing)
+        return calls
 
     @staticmethod
     def _refuse(name, t, size, dtype, device):
@@ -342,7 +346,7 @@ class loader:
         if device is None:
             st = call(*args)
         else:
-            with loader._torch_cuda.device(device):
+            with loader._cuda[2].device(device):
                 st = call(*args)
         if st != 0:
             _check(st)
