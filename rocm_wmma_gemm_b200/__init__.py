@@ -287,6 +287,19 @@ class loader:
         return TYPE_PAIRS[pair]
 
     _TORCH_NAMES = {"f16": "float16", "bf16": "bfloat16", "f32": "float32"}
+    _PAIR_DTYPES = None  # type index -> torch's (output, input) dtypes, filled on first use
+
+    @staticmethod
+    def _dtypes(t):
+        """torch's (output, input) dtypes of type pair t, for calls that name their types: some arguments
+        may be addresses, and the tensors among the others must still hold what the kernels read."""
+        if loader._PAIR_DTYPES is None:
+            try:
+                import torch
+            except ImportError:
+                return None, None  # (so no argument is a tensor)
+            loader._PAIR_DTYPES = {i: tuple(getattr(torch, loader._TORCH_NAMES[n]) for n in pair) for pair, i in TYPE_PAIRS.items()}
+        return loader._PAIR_DTYPES[t]
 
     def _arguments(self, stream, spec):
         """(device to make current or None, stream cell, addresses) of a call's array arguments.
@@ -384,7 +397,7 @@ class loader:
         the sum over them), N or more gives each its own."""
         t = self._types_of(C, A, types)
         mn, vec = batch_count * M * N, N + (batch_count - 1) * bias_stride if N else 0
-        ct, it = getattr(C, "dtype", None), getattr(A, "dtype", None)
+        ct, it = (C.dtype, A.dtype) if types is None else self._dtypes(t)
         dev, sp, (c, a, b, bi, re, pr, bg) = self._arguments(stream, (
             ("C", C, mn, None), ("A", A, batch_count * M * K, None), ("B", B, batch_count * K * N, it),
             ("bias", bias, vec, ct), ("residual", residual, mn, ct), ("preact", preact, mn, ct),
@@ -401,7 +414,8 @@ class loader:
         left as they are.  bias and bias_grad are groups x N.  The input gradient is the same call
         on the output's gradient with layout_b flipped and N and K exchanged."""
         t = self._types_of(C, A, types)
-        mn, ct, it = rows * N, getattr(C, "dtype", None), getattr(A, "dtype", None)
+        mn = rows * N
+        ct, it = (C.dtype, A.dtype) if types is None else self._dtypes(t)
         dev, sp, (c, a, b, bi, re, pr, bg, off) = self._arguments(stream, (
             ("C", C, mn, None), ("A", A, rows * K, None), ("B", B, groups * K * N, it),
             ("bias", bias, groups * N, ct), ("residual", residual, mn, ct), ("preact", preact, mn, ct),
@@ -418,7 +432,7 @@ class loader:
         An empty group's C_e is zero."""
         t = self._types_of(C, A, types)
         dev, sp, (c, a, b, off) = self._arguments(stream, (
-            ("C", C, groups * M * N, None), ("A", A, rows * M, None), ("B", B, rows * N, getattr(A, "dtype", None)),
+            ("C", C, groups * M * N, None), ("A", A, rows * M, None), ("B", B, rows * N, A.dtype if types is None else self._dtypes(t)[1]),
             ("offsets", offsets, groups + 1, self._torch_type(offsets, "int32"))))
         self._on(dev, self._lib.b200_gemm_grouped_wgrad, t, c, a, b, off, rows, M, N, groups, int(layout_c),
                  int(accumulate), sp)
@@ -440,7 +454,7 @@ class loader:
                 raise ValueError(f"dY is {getattr(dY, 'dtype', 'an address')}: a float16, bfloat16 or float32 tensor, or give types")
         else:
             t = self._types_of(dY, None, types)
-        mn, ct = batch_count * M * N, getattr(dY, "dtype", None)
+        mn, ct = batch_count * M * N, dY.dtype if types is None else self._dtypes(t)[0]
         vec = groups * N if groups else (N + (batch_count - 1) * bias_stride if N else 0)
         dev, sp, (dz, dy, z, bg, off) = self._arguments(stream, (
             ("dZ", dZ, mn, ct), ("dY", dY, mn, None), ("preact", preact, mn, ct),

@@ -55,3 +55,43 @@ def test_first_calls_of_two_threads(gemm_lib, monkeypatch, at):
     monkeypatch.setattr(torch, "_C", Calls())
     call()
     assert not errors and len(results) == 2 and set(results) == {None}, errors
+
+
+C, A, B, SIDE, OFF = [0x10000000 * (i + 1) for i in range(5)]  # addresses, never dereferenced
+
+
+@pytest.mark.parametrize("types,out,inp", [(("f32", "bf16"), "float32", "bfloat16"), (0, "float16", "float16")])
+def test_tensors_beside_addresses(gemm_lib, monkeypatch, types, out, inp):
+    """With some arguments given as addresses, the tensors among the others still have the types that
+    the call takes: a narrower one would end before the kernels do."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("stand-in addresses: only for processes without a GPU")
+    L = gemm_lib.loader()
+    monkeypatch.setattr(gemm_lib.loader, "_cuda", (lambda index: 0, lambda: 0, torch.cuda))
+    other = {torch.float32: torch.bfloat16, torch.float16: torch.float32, torch.bfloat16: torch.uint8}
+    co, io = getattr(torch, out), getattr(torch, inp)
+    bad_c, bad_i = Tensor(other[co]), Tensor(other[io])
+    calls = [
+        lambda: L.gemm_fused(C, A, bad_i, 8, 8, 8, types=types),
+        lambda: L.gemm_fused(C, A, B, 8, 8, 8, bias=bad_c, types=types),
+        lambda: L.gemm_fused(C, A, B, 8, 8, 8, residual=bad_c, types=types),
+        lambda: L.gemm_fused(C, A, B, 8, 8, 8, preact=bad_c, types=types),
+        lambda: L.gemm_fused(C, Tensor(io), B, 8, 8, 8, residual=bad_c, types=types),
+        lambda: L.gemm_grouped(C, A, bad_i, OFF, 8, 8, 8, 1, types=types),
+        lambda: L.gemm_grouped(C, A, B, OFF, 8, 8, 8, 1, bias=bad_c, types=types),
+        lambda: L.gemm_grouped(C, A, B, OFF, 8, 8, 8, 1, preact=bad_c, gradient=True, activation="relu", types=types),
+        lambda: L.gemm_grouped_wgrad(C, A, bad_i, OFF, 8, 8, 8, 1, types=types),
+        lambda: L.activation_backward(bad_c, A, B, 8, 8, activation="relu", types=types),
+        lambda: L.activation_backward(C, A, bad_c, 8, 8, activation="relu", types=types),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match="is torch"):
+            call()
+            pytest.fail(f"call {i} was taken")
+    ok = [lambda: L.gemm_fused(C, A, Tensor(io, address=B), 8, 8, 8, bias=Tensor(co, address=SIDE), types=types),
+          lambda: L.gemm_grouped_wgrad(C, A, Tensor(io, address=B), OFF, 8, 8, 8, 1, types=types),
+          lambda: L.activation_backward(C, A, Tensor(co, address=SIDE), 8, 8, activation="relu", types=types)]
+    for call in ok:  # accepted: all that stops these is the missing device
+        with pytest.raises(gemm_lib.GemmError, match="no CUDA device"):
+            call()
