@@ -275,7 +275,9 @@ int b200_gemm_slab_host(b200_gemm_comm* comm, int types, void* C_slab, const voi
  * The calls are asynchronous on `*stream`, on the current device, and may be captured into a
  * graph after the first call on the device.  A call that needs scratch memory (bias gradients, K
  * partitions, operands that have to be padded) keeps it per stream and lets it grow on demand; a
- * captured call's scratch belongs to the graph.  Calls that overlap on the GPU must not share
+ * captured call's scratch belongs to the graph.  A stream may be destroyed with such calls pending; its
+ * scratch (up to the padded copies of a call's operands) stays allocated, for a later stream with the
+ * same handle.  Calls that overlap on the GPU must not share
  * outputs.  Host threads may use one stream: calls that need scratch memory queue one after the other.
  *
  * Refused before anything runs: bad layouts, sizes, activations (BAD_LAYOUT, BAD_SIZE, BAD_CONFIG),

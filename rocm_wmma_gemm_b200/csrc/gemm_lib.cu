@@ -176,7 +176,12 @@ struct DeviceCtx {
         float*       ptr;
         size_t       bytes;
         int          kind; // WS_SPLIT_K or WS_EPILOGUE: a call may use one of each
-        const void*  thread; // the per-thread default stream is one handle for many streams: whose (else nullptr)
+        // The per-thread default stream is one handle for many streams: whose (else nullptr), and the stream's
+        // id, since a thread that has ended may leave its address to another and its work pending.  (A
+        // destroyed stream's handle comes back only after its work has completed, as its other
+        // resources do.)
+        const void*        thread;
+        unsigned long long id;
     };
     std::vector<Workspace> workspaces;
     // buffers a workspace has outgrown: freed once the work that was queued on them has drained
@@ -327,6 +332,8 @@ static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, floa
 {
     static thread_local char t_self;
     const void* const        thread = stream == cudaStreamPerThread ? &t_self : nullptr;
+    unsigned long long       id     = 0;
+    if (thread) CUDA_TRY(cudaStreamGetId(stream, &id));
     std::lock_guard<std::mutex> lock(ctx->ws_mutex);
     for (size_t i = 0; i < ctx->retired.size();) {
         if (cudaEventQuery(ctx->retired[i].drained) == cudaSuccess) {
@@ -341,7 +348,16 @@ static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, floa
     }
     for (auto& w : ctx->workspaces) {
         if (w.stream != stream || w.kind != kind || w.thread != thread) continue;
-        if (w.bytes < bytes) {
+        if (w.id != id) {
+            // The last kernels of the thread that has ended may still be using the buffer, and nothing can be
+            // recorded behind them any more.  cudaFree waits for all work on the device.
+            cudaFree(w.ptr);
+            w.ptr   = nullptr;
+            w.bytes = 0;
+            w.id    = id;
+            CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&w.ptr), bytes));
+            w.bytes = bytes;
+        } else if (w.bytes < bytes) {
             const size_t want  = bytes + bytes / 4;
             float*       fresh = nullptr;
             CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&fresh), want));
@@ -361,7 +377,7 @@ static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, floa
         *out = w.ptr;
         return B200_GEMM_OK;
     }
-    DeviceCtx::Workspace w{stream, nullptr, 0, kind, thread};
+    DeviceCtx::Workspace w{stream, nullptr, 0, kind, thread, id};
     CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&w.ptr), bytes));
     w.bytes = bytes;
     ctx->workspaces.push_back(w);
