@@ -324,6 +324,18 @@ static int get_ctx(DeviceCtx** out)
     return B200_GEMM_OK;
 }
 
+// While it lives, this thread may allocate and query although another thread captures a stream in the
+// mode that forbids it (nothing done here belongs into that capture, which would be invalidated).
+struct BesideCaptures {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    bool                  set;
+    BesideCaptures() : set(cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess) {}
+    ~BesideCaptures()
+    {
+        if (set) (void)cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+};
+
 // Split-K workspace of at least `bytes` for `stream`: cached per stream and grown on demand, so
 // the steady state allocates nothing (an allocation per call costs more than a skinny GEMM).
 // A buffer that has become too small is not freed here - kernels queued on the stream may still
@@ -335,6 +347,12 @@ static int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, floa
     unsigned long long       id     = 0;
     if (thread) CUDA_TRY(cudaStreamGetId(stream, &id));
     std::lock_guard<std::mutex> lock(ctx->ws_mutex);
+    for (auto& w : ctx->workspaces) // the steady state
+        if (w.stream == stream && w.kind == kind && w.thread == thread && w.id == id && w.bytes >= bytes && ctx->retired.empty()) {
+            *out = w.ptr;
+            return B200_GEMM_OK;
+        }
+    const BesideCaptures relaxed;
     for (size_t i = 0; i < ctx->retired.size();) {
         if (cudaEventQuery(ctx->retired[i].drained) == cudaSuccess) {
             cudaFree(ctx->retired[i].ptr);

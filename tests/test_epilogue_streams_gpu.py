@@ -103,3 +103,33 @@ def test_threads_that_end_with_calls_pending(L, delay):
     assert not errors, errors
     for w in todo:
         w.check()
+
+
+def test_first_call_of_a_stream_beside_a_capture(L):
+    """Scratch is allocated while another thread captures (in the mode that forbids other threads'
+    allocations): neither the call nor the capture fails."""
+    mine, other = Work(1, 320, 264, 333), Work(2, 900, 520, 777)
+    mine.call(L)
+    torch.cuda.synchronize()
+    stream, errors = torch.cuda.Stream(), []
+
+    def call():
+        try:
+            with torch.cuda.stream(stream):
+                other.call(L)
+        except Exception as e:  # noqa: BLE001 (reported below)
+            errors.append(e)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="global"):
+        mine.call(L)
+        t = threading.Thread(target=call)
+        t.start()
+        t.join()
+        mine.call(L)
+    assert not errors, errors
+    mine.c.fill_(float("nan"))
+    graph.replay()
+    torch.cuda.synchronize()
+    mine.check()
+    other.check()
