@@ -273,7 +273,8 @@ int b200_gemm_slab_host(b200_gemm_comm* comm, int types, void* C_slab, const voi
  * matrices of C's shape, layout and batch stride.
  *
  * The calls are asynchronous on `*stream`, on the current device, and may be captured into a
- * graph after the first call on the device.  A call that needs scratch memory (bias gradients, K
+ * graph after the first call of any kind on the device; the first of these calls loads their kernels
+ * (15 ms).  A call that needs scratch memory (bias gradients, K
  * partitions, operands that have to be padded) keeps it per stream and lets it grow on demand; a
  * captured call's scratch belongs to the graph.  A stream may be destroyed with such calls pending; its
  * scratch (up to the padded copies of a call's operands) stays allocated, for a later stream with the

@@ -165,7 +165,8 @@ struct DeviceCtx {
     std::atomic<bool> ready{false}; // set last, read first: initialised contexts skip the lock
     int           sm_count = 0;
     PairCache     pairs;
-    int           epilogue_pairs = 0; // co-resident CTA pairs of the kernels with an epilogue
+    std::atomic<bool> epilogues_ready{false}; // the kernels with an epilogue are loaded (epilogue_ctx)
+    int           epilogue_pairs = 0; // co-resident CTA pairs of these kernels
     unsigned int* d_status = nullptr;
     // split-K workspaces, one per stream that has used split-K (calls on one stream are ordered,
     // so they can share a buffer; calls on different streams must not).  A call holds its stream's lock
@@ -281,8 +282,6 @@ static cudaError_t set_all_kernel_attributes()
     return e;
 }
 
-static int prepare_epilogues(DeviceCtx* ctx); // epilogue_driver.inc
-
 static int get_ctx(DeviceCtx** out)
 {
     int         dev = -1;
@@ -316,8 +315,6 @@ static int get_ctx(DeviceCtx** out)
         CUDA_TRY(cudaMalloc(&c.d_status, sizeof(unsigned int)));
         CUDA_TRY(cudaMemset(c.d_status, 0, sizeof(unsigned int)));
         CUDA_TRY(set_all_kernel_attributes());
-        const int st = prepare_epilogues(&c);
-        if (st != B200_GEMM_OK) return st;
         c.ready.store(true, std::memory_order_release);
     }
     *out = &c;

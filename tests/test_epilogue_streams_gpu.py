@@ -133,3 +133,34 @@ def test_first_call_of_a_stream_beside_a_capture(L):
     torch.cuda.synchronize()
     mine.check()
     other.check()
+
+
+FIRST = """
+import sys; sys.path.insert(0, {root!r}); sys.path.insert(0, {tests!r})
+import torch, rocm_wmma_gemm_b200 as g
+from test_epilogue_streams_gpu import Work
+L, w = g.loader(), Work(3, 320, 264, 333)
+x = torch.ones(64, 64, device="cuda", dtype=torch.bfloat16)
+L.gemm(torch.empty_like(x), x, x, 64, 64, 64)  # the plain product only
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, capture_error_mode="global"):
+    w.call(L)
+    L.activation_backward(w.c, w.z, w.z, w.M, w.N, activation="gelu")
+    w.call(L)
+graph.replay()
+torch.cuda.synchronize()
+w.check()
+g.device_status()
+print("fine")
+"""
+
+
+def test_first_call_is_captured(L):
+    """A process that has made plain products only captures its first calls with an epilogue."""
+    import os
+    import subprocess
+    import sys
+    tests = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST.format(root=os.path.dirname(tests), tests=tests)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
