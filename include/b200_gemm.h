@@ -308,9 +308,11 @@ typedef struct b200_gemm_epilogue {
                                 bias and bias_grad are groups x N. */
 } b200_gemm_epilogue;
 
-/* C = A*B with an epilogue (epi NULL: none).  Arguments as in b200_gemm_ex.  M, N, K, batch of 0:
- * empty C is left alone, a bias gradient over no rows is zero, K == 0 is a product of zeros
- * (the epilogue still applies).  The plan is that of b200_gemm_ex for the same problem. */
+/* C = A*B with an epilogue (epi NULL: none).  Arguments as in b200_gemm_ex; batch_count is at least 1.
+ * With M or N of 0 C is left alone and a bias gradient over no rows is zero; K == 0 is a product of zeros
+ * (the epilogue still applies).  The plan starts from that of b200_gemm_ex for the same problem, but
+ * tile widths and K partitions may differ, and sizes that TMA cannot address run on padded copies of
+ * the operands. */
 int b200_gemm_fused(int types, void* C, const void* A, const void* B, size_t M, size_t N, size_t K,
                     size_t batch_count, int layout_c, int layout_a, int layout_b, void* stream,
                     const b200_gemm_epilogue* epi);
