@@ -613,12 +613,15 @@ struct EpilogueMaps {
     CUtensorMap in, aux;
 };
 
-// Sum of v[j] over the 32 lanes, for N = 16 or 32 values of j: lane l receives the sum of v[l % N].
-template <int N>
-__device__ __forceinline__ float warp_column_sums(float (&v)[N], uint32_t lane)
+// The epilogues work in pieces of 16 columns, in loops that are not unrolled: the whole of a piece - bias, activation, residual, conversion - is a few
+// hundred instructions, which stay in the instruction cache.
+constexpr int PIECE = 16;
+
+// Sum of v[j] over the 32 lanes: lane l receives the sum of v[l % PIECE].
+__device__ __forceinline__ float warp_column_sums(float (&v)[PIECE], uint32_t lane)
 {
 #pragma unroll
-    for (int s = N / 2; s > 0; s /= 2) {
+    for (int s = PIECE / 2; s > 0; s /= 2) {
         const bool up = (lane & s) != 0u;
 #pragma unroll
         for (int i = 0; i < s; ++i) {
@@ -627,25 +630,12 @@ __device__ __forceinline__ float warp_column_sums(float (&v)[N], uint32_t lane)
             v[i]             = keep + __shfl_xor_sync(0xffffffffu, send, s);
         }
     }
-    if constexpr (N == 16) return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
-    else return v[0];
-}
-
-// The epilogues work in pieces of 16 columns, in loops that are not unrolled: the whole of a piece - bias, activation, residual, conversion - is a few
-// hundred instructions, which stay in the instruction cache.
-constexpr int PIECE = 16, COLUMN_PIECE = 16;
-
-template <int N>
-__device__ __forceinline__ void tmem_ld_piece(uint32_t addr, uint32_t (&r)[N])
-{
-    if constexpr (N == 32) ptx::tmem_ld_32x32(addr, r);
-    else ptx::tmem_ld_32x16(addr, r);
+    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], PIECE);
 }
 
 // Accumulator columns from TMEM.  The load and its wait stay together: a load in flight across a
 // branch or a loop's back edge would let the compiler copy its destination registers, and reuse
 // them, before the hardware has written them.
-template <int N>
 struct TmemPieces {
     uint32_t addr;  // first column of the chunk
     uint32_t count; // pieces
@@ -653,17 +643,17 @@ struct TmemPieces {
 
     // Piece i (in order); `done` is called once the chunk's last piece has been read.
     template <class F>
-    __device__ __forceinline__ void get(uint32_t i, float (&v)[N], F&& done)
+    __device__ __forceinline__ void get(uint32_t i, float (&v)[PIECE], F&& done)
     {
         if (empty) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = 0.f;
+            for (int j = 0; j < PIECE; ++j) v[j] = 0.f;
         } else {
-            uint32_t t[N];
-            tmem_ld_piece(addr + i * N, t);
+            uint32_t t[PIECE];
+            ptx::tmem_ld_32x16(addr + i * PIECE, t);
             ptx::tmem_ld_wait(t);
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = __uint_as_float(t[j]);
+            for (int j = 0; j < PIECE; ++j) v[j] = __uint_as_float(t[j]);
         }
         if (i + 1u == count) done();
     }
@@ -671,7 +661,6 @@ struct TmemPieces {
 
 // Sums of a cluster's K partitions: this CTA's own part from TMEM, the others' from shared memory
 // (laid out [16-byte unit][lane], see the cluster exchange), added in partition order.
-template <int N>
 struct ClusterPieces {
     uint32_t addr;       // this CTA's accumulator columns of the chunk
     uint32_t ring;       // partial of partition 0 of this chunk, this warp's rows, this lane
@@ -679,23 +668,23 @@ struct ClusterPieces {
     uint32_t parts, rank;
 
     template <class F>
-    __device__ __forceinline__ void get(uint32_t i, float (&v)[N], F&&) const
+    __device__ __forceinline__ void get(uint32_t i, float (&v)[PIECE], F&&) const
     {
-        uint32_t own[N];
-        tmem_ld_piece(addr + i * N, own);
+        uint32_t own[PIECE];
+        ptx::tmem_ld_32x16(addr + i * PIECE, own);
         ptx::tmem_ld_wait(own);
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = 0.f;
+        for (int j = 0; j < PIECE; ++j) v[j] = 0.f;
 #pragma unroll 1
         for (uint32_t s = 0; s < parts; ++s) {
             if (s == rank) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) v[j] += __uint_as_float(own[j]);
+                for (int j = 0; j < PIECE; ++j) v[j] += __uint_as_float(own[j]);
             } else {
 #pragma unroll
-                for (uint32_t u = 0; u < N / 4; ++u) {
+                for (uint32_t u = 0; u < PIECE / 4; ++u) {
                     uint32_t x[4];
-                    ptx::ld_shared_v4(ring + s * slot_bytes + (i * (N / 4) + u) * 512u, x[0], x[1], x[2], x[3]);
+                    ptx::ld_shared_v4(ring + s * slot_bytes + (i * (PIECE / 4) + u) * 512u, x[0], x[1], x[2], x[3]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) v[4 * u + k] += __uint_as_float(x[k]);
                 }
@@ -1093,17 +1082,17 @@ struct EpilogueColumns {
         return (static_cast<uint64_t>(c.z_out) * p.N + col) * p.M + i;
     }
 
-    __device__ __forceinline__ void load_side(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, float (&side)[COLUMN_PIECE]) const
+    __device__ __forceinline__ void load_side(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, float (&side)[PIECE]) const
     {
         const T* src = static_cast<const T*>(ep.gradient ? ep.preact : ep.residual);
 #pragma unroll
-        for (uint32_t r = 0; r < COLUMN_PIECE; ++r) side[r] = live && r < n ? to_f32(src[at(c, col0 + r, i)]) : 0.f;
+        for (uint32_t r = 0; r < PIECE; ++r) side[r] = live && r < n ? to_f32(src[at(c, col0 + r, i)]) : 0.f;
     }
 
     // Bias gradients: the piece's sum over the columns is added to `row_sum`, its sums over the rows go
     // to row `block_rows` of the partial sums.
     __device__ __forceinline__ void finish(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, uint32_t block_rows,
-                                           float (&v)[COLUMN_PIECE], const float (&side)[COLUMN_PIECE], float& row_sum) const
+                                           float (&v)[PIECE], const float (&side)[PIECE], float& row_sum) const
     {
         if (ep.gradient) {
             if (ep.streamed)
@@ -1114,16 +1103,16 @@ struct EpilogueColumns {
                 if (ep.bias_on_rows) {
                     const float b = live ? to_f32(bias[i]) : 0.f;
 #pragma unroll
-                    for (int r = 0; r < COLUMN_PIECE; ++r) v[r] += b;
+                    for (int r = 0; r < PIECE; ++r) v[r] += b;
                 } else {
 #pragma unroll
-                    for (uint32_t r = 0; r < COLUMN_PIECE; ++r) v[r] += r < n ? to_f32(bias[col0 + r]) : 0.f;
+                    for (uint32_t r = 0; r < PIECE; ++r) v[r] += r < n ? to_f32(bias[col0 + r]) : 0.f;
                 }
             }
             if (ep.aux && live) {
                 T* pre = static_cast<T*>(ep.preact);
 #pragma unroll
-                for (uint32_t r = 0; r < COLUMN_PIECE; ++r)
+                for (uint32_t r = 0; r < PIECE; ++r)
                     if (r < n) pre[at(c, col0 + r, i)] = from_f32<T>(v[r]);
             }
             apply_activation(ep, v);
@@ -1132,16 +1121,16 @@ struct EpilogueColumns {
         if (live) {
             T* out = static_cast<T*>(p.out);
 #pragma unroll
-            for (uint32_t r = 0; r < COLUMN_PIECE; ++r)
+            for (uint32_t r = 0; r < PIECE; ++r)
                 if (r < n) out[at(c, col0 + r, i)] = from_f32<T>(v[r]);
         }
         if (!ep.part) return;
         if (ep.bias_on_rows) {
 #pragma unroll
-            for (uint32_t r = 0; r < COLUMN_PIECE; ++r) row_sum += r < n ? v[r] : 0.f;
+            for (uint32_t r = 0; r < PIECE; ++r) row_sum += r < n ? v[r] : 0.f;
         } else {
 #pragma unroll
-            for (int r = 0; r < COLUMN_PIECE; ++r) v[r] = live ? v[r] : 0.f;
+            for (int r = 0; r < PIECE; ++r) v[r] = live ? v[r] : 0.f;
             const float sum = warp_column_sums(v, lane);
             if (lane < n) ep.part[static_cast<uint64_t>(block_rows) * p.N + col0 + lane] = sum;
         }
@@ -1151,16 +1140,16 @@ struct EpilogueColumns {
     // piece, loaded before the accumulator was awaited.
     template <class Pieces, class F>
     __device__ __forceinline__ void chunk(const WorkCoord& c, uint32_t col0, uint32_t n, uint32_t i, bool live, uint32_t block,
-                                          uint32_t block_rows, Pieces& pieces, uint32_t npieces, float (&side)[COLUMN_PIECE], F&& accumulators_read) const
+                                          uint32_t block_rows, Pieces& pieces, uint32_t npieces, float (&side)[PIECE], F&& accumulators_read) const
     {
         float row_sum = 0.f;
 #pragma unroll 1
         for (uint32_t pc = 0; pc < npieces; ++pc) {
-            const uint32_t m = n > pc * COLUMN_PIECE ? min(n - pc * COLUMN_PIECE, static_cast<uint32_t>(COLUMN_PIECE)) : 0u;
-            float          v[COLUMN_PIECE];
-            if (pc > 0u && ep.streamed) load_side(c, col0 + pc * COLUMN_PIECE, m, i, live, side);
+            const uint32_t m = n > pc * PIECE ? min(n - pc * PIECE, static_cast<uint32_t>(PIECE)) : 0u;
+            float          v[PIECE];
+            if (pc > 0u && ep.streamed) load_side(c, col0 + pc * PIECE, m, i, live, side);
             pieces.get(pc, v, accumulators_read);
-            if (m) finish(c, col0 + pc * COLUMN_PIECE, m, i, live, block_rows, v, side, row_sum);
+            if (m) finish(c, col0 + pc * PIECE, m, i, live, block_rows, v, side, row_sum);
         }
         if (ep.part && ep.bias_on_rows && live && n) ep.part[static_cast<uint64_t>(block) * p.M + i] = row_sum;
     }
@@ -1215,7 +1204,7 @@ struct EpilogueTransposed {
 
     // Columns [col0, min(col0 + 32, stop)) are the group's.  False: a wait ran out.
     template <class F>
-    __device__ __forceinline__ bool chunk(const WorkCoord& c, uint32_t row0, uint32_t col0, uint32_t stop, float bias, TmemPieces<COLUMN_PIECE>& pieces, F&& accumulators_read)
+    __device__ __forceinline__ bool chunk(const WorkCoord& c, uint32_t row0, uint32_t col0, uint32_t stop, float bias, TmemPieces& pieces, F&& accumulators_read)
     {
         const uint32_t b    = slot(0);
         const uint32_t sbuf = stg + b * BUF, xbuf = stg + ep.bufs * BUF, at = lane * static_cast<uint32_t>(sizeof(T));
@@ -1234,30 +1223,30 @@ struct EpilogueTransposed {
         __syncwarp();
         float row_sum = 0.f;
 #pragma unroll 1
-        for (uint32_t pc = 0; pc < 32u / COLUMN_PIECE; ++pc) {
-            const uint32_t first = pc * COLUMN_PIECE, to = sbuf + first * LINE + at;
-            float          v[COLUMN_PIECE], side[COLUMN_PIECE];
+        for (uint32_t pc = 0; pc < 32u / PIECE; ++pc) {
+            const uint32_t first = pc * PIECE, to = sbuf + first * LINE + at;
+            float          v[PIECE], side[PIECE];
             pieces.get(pc, v, accumulators_read);
             if (ep.streamed)
 #pragma unroll
-                for (uint32_t j = 0; j < COLUMN_PIECE; ++j) side[j] = to_f32(ld_shared_elem<T>(to + j * LINE));
+                for (uint32_t j = 0; j < PIECE; ++j) side[j] = to_f32(ld_shared_elem<T>(to + j * LINE));
             if (ep.gradient) {
                 if (ep.streamed) apply_slope(ep, v, side);
             } else {
                 if (ep.bias)
 #pragma unroll
-                    for (uint32_t j = 0; j < COLUMN_PIECE; ++j) v[j] += bias;
+                    for (uint32_t j = 0; j < PIECE; ++j) v[j] += bias;
                 if (ep.aux)
 #pragma unroll
-                    for (uint32_t j = 0; j < COLUMN_PIECE; ++j) st_shared_elem(xbuf + (first + j) * LINE + at, from_f32<T>(v[j]));
+                    for (uint32_t j = 0; j < PIECE; ++j) st_shared_elem(xbuf + (first + j) * LINE + at, from_f32<T>(v[j]));
                 apply_activation(ep, v);
                 if (ep.streamed) add_values(v, side);
             }
 #pragma unroll
-            for (uint32_t j = 0; j < COLUMN_PIECE; ++j) st_shared_elem(to + j * LINE, from_f32<T>(v[j]));
+            for (uint32_t j = 0; j < PIECE; ++j) st_shared_elem(to + j * LINE, from_f32<T>(v[j]));
             if (ep.part)
 #pragma unroll
-                for (uint32_t j = 0; j < COLUMN_PIECE; ++j) row_sum += col0 + first + j < stop ? v[j] : 0.f;
+                for (uint32_t j = 0; j < PIECE; ++j) row_sum += col0 + first + j < stop ? v[j] : 0.f;
         }
         const uint32_t row = row0 + lane;
         if (ep.part && row < p.M)
@@ -1869,7 +1858,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                 if (mine == 0u) release(buf);
 #pragma unroll 1
                 for (uint32_t k = 0; k < mine; ++k) {
-                    TmemPieces<COLUMN_PIECE> pieces{tacc + (hw + EPI_SETS * k) * 32u, 32u / COLUMN_PIECE, c.kb1 == c.kb0};
+                    TmemPieces pieces{tacc + (hw + EPI_SETS * k) * 32u, 32u / PIECE, c.kb1 == c.kb0};
                     if (epp->streamed && k > 0u && k - 1u + epp->bufs < mine) {
                         et.buffers_free(); // the chunk before this one left from the buffer asked for now
                         et.request(epp->bufs - 1u, row0, col(k - 1u + epp->bufs));
@@ -1894,15 +1883,15 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                 for (uint32_t ch = hw; ch < CHUNKS; ch += EPI_SETS) {
                     const uint32_t col0 = c.n0 + ch * 32u;
                     const uint32_t n    = col0 < c.end ? min(min(32u, BN - ch * 32u), c.end - col0) : 0u;
-                    constexpr uint32_t NP = (BN < 32 ? BN : 32) / COLUMN_PIECE; // pieces of a chunk
-                    float          side[COLUMN_PIECE];
-                    if (epp->streamed) ec.load_side(c, col0, min(n, static_cast<uint32_t>(COLUMN_PIECE)), i, live, side);
+                    constexpr uint32_t NP = (BN < 32 ? BN : 32) / PIECE; // pieces of a chunk
+                    float          side[PIECE];
+                    if (epp->streamed) ec.load_side(c, col0, min(n, static_cast<uint32_t>(PIECE)), i, live, side);
                     if (!seen) {
                         ok = accumulator(buf, (it / NUM_ACC) & 1u);
                         if (!ok) break;
                         seen = true;
                     }
-                    TmemPieces<COLUMN_PIECE> pieces{tacc + ch * 32u, NP, c.kb1 == c.kb0};
+                    TmemPieces pieces{tacc + ch * 32u, NP, c.kb1 == c.kb0};
                     const uint32_t block = epp->ragged == RAGGED_ROWS
                                                ? group_first_block(c.first, c.group, bs) + (col0 - c.first) / bs
                                                : c.z_out * epp->part_blocks + col0 / bs;
@@ -1955,7 +1944,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                             ew.finish_plain(c, row0, col(k), c.end, tacc + (hw + EPI_SETS * k) * EW::CH, c.kb1 == c.kb0, read);
                             continue;
                         }
-                        TmemPieces<PIECE> pieces{tacc + (hw + EPI_SETS * k) * EW::CH, EW::CH / PIECE, c.kb1 == c.kb0};
+                        TmemPieces pieces{tacc + (hw + EPI_SETS * k) * EW::CH, EW::CH / PIECE, c.kb1 == c.kb0};
                         if (epp->streamed && k > 0u && k - 1u + epp->bufs < mine) {
                             ew.buffers_free(); // the chunk before this one left from the buffer asked for now
                             ew.request(epp->bufs - 1u, row0, col(k - 1u + epp->bufs), c.z_out);
@@ -2212,7 +2201,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
 #pragma unroll 1
             for (uint32_t ch = krank + (EP ? hw * ks : 0u); ch < static_cast<uint32_t>(NCH); ch += (EP ? EPI_SETS : 1u) * ks) {
                 if constexpr (EP) {
-                    ClusterPieces<TR ? COLUMN_PIECE : PIECE> pieces{tacc + ch * O_CH, ring + ((ch / ks) * ks * 4u + q) * WSLOT + lane * 16u, 4u * WSLOT, ks, krank};
+                    ClusterPieces pieces{tacc + ch * O_CH, ring + ((ch / ks) * ks * 4u + q) * WSLOT + lane * 16u, 4u * WSLOT, ks, krank};
                     dep_wait();
                     if constexpr (TR) {
                         const EpilogueColumns<OUT> ec{p, *epp, lane};
@@ -2221,10 +2210,10 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         const uint32_t col0 = ks_c.n0 + ch * 32u;
                         const uint32_t bs   = BN < 32 ? BN : 32;
                         const uint32_t n    = col0 < p.N ? min(min(32u, BN - ch * 32u), p.N - col0) : 0u;
-                        float          side[COLUMN_PIECE];
-                        if (epp->streamed) ec.load_side(ks_c, col0, min(n, static_cast<uint32_t>(COLUMN_PIECE)), i, live, side);
+                        float          side[PIECE];
+                        if (epp->streamed) ec.load_side(ks_c, col0, min(n, static_cast<uint32_t>(PIECE)), i, live, side);
                         ec.chunk(ks_c, col0, n, i, live, ks_c.z_out * epp->part_blocks + col0 / bs,
-                                 ks_c.z_out * epp->part_blocks + ks_c.m0 / p.bm * 4u + q, pieces, bs / COLUMN_PIECE, side, [] {});
+                                 ks_c.z_out * epp->part_blocks + ks_c.m0 / p.bm * 4u + q, pieces, bs / PIECE, side, [] {});
                     } else {
                         const uint32_t col0 = ks_c.n0 + ch * O_CH;
                         if (row_live && col0 < p.N) {
