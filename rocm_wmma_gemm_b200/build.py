@@ -54,12 +54,12 @@ def is_stale(path: str = LIB_PATH) -> bool:
     return any(os.path.getmtime(d) > t for d in DEPENDS if os.path.exists(d))
 
 
-def _compile(out: str, extra: list, verbose: bool) -> str:
+def _compile(out: str, extra: list, verbose: bool, sources: list = SOURCES) -> str:
     # one object per source, compiled side by side, then linked
     with tempfile.TemporaryDirectory() as tmp:
-        objects = [os.path.join(tmp, os.path.basename(src) + ".o") for src in SOURCES]
+        objects = [os.path.join(tmp, os.path.basename(src) + ".o") for src in sources]
         cmds = [[_nvcc()] + NVCC_FLAGS + extra + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", o, src]
-                for o, src in zip(objects, SOURCES)]
+                for o, src in zip(objects, sources)]
         procs = [subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for cmd in cmds]
         outputs = [p.communicate()[0] for p in procs]
         cmds.append([_nvcc()] + NVCC_FLAGS[:2] + ["-shared", "-o", out] + objects + ["-ldl"])
@@ -86,7 +86,8 @@ def build_timeline(force: bool = False, verbose: bool = False) -> str:
     """Compile the timeline (profiling) variant of the library; returns its path."""
     if not force and not is_stale(TIMELINE_LIB_PATH):
         return TIMELINE_LIB_PATH
-    return _compile(TIMELINE_LIB_PATH, ["-DB200_GEMM_TIMELINE"], verbose)
+    # (gemm_lib.cu includes epilogue_kernels.cu in this variant: all stamps go to one set of variables)
+    return _compile(TIMELINE_LIB_PATH, ["-DB200_GEMM_TIMELINE"], verbose, SOURCES[:1])
 
 
 if __name__ == "__main__":

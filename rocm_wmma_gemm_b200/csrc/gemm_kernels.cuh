@@ -1815,7 +1815,18 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
             if (s_seen[at] == 0u) return false;
             (void)ptx::mbar_test_wait(ptx::smem_u32(&s_tfull[bar_i]), parity); // (completed: orders this warp behind it too)
             ptx::tc_fence_after();
+            if (warp == 2u && lane == 0 && waits == 1u) {
+                B200_TL(9);
+                B200_TL_CTA(2);
+            }
             return true;
+        };
+        [[maybe_unused]] uint32_t nstore = 0;
+        auto stored = [&] { // (timeline) a chunk's stores have been issued
+            if (warp == 2u && lane == 0) {
+                if (nstore++ == 0u) B200_TL(10);
+                B200_TL(11);
+            }
         };
         if constexpr (KS) {
             // one tile per cluster; the partials are summed after the cluster barriers below
@@ -1864,6 +1875,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         et.request(epp->bufs - 1u, row0, col(k - 1u + epp->bufs));
                     }
                     live_warp = et.chunk(c, row0, col(k), stop, bias, pieces, [&] { if (k + 1u == mine) release(buf); });
+                    stored();
                     if (!live_warp) break; // (a wait ran out: the abort flag ends the other roles)
                 }
             }
@@ -1942,6 +1954,7 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                         auto read = [&] { if (k + 1u == mine) release(bar_i); };
                         if (epp->plain) {
                             ew.finish_plain(c, row0, col(k), c.end, tacc + (hw + EPI_SETS * k) * EW::CH, c.kb1 == c.kb0, read);
+                            stored();
                             continue;
                         }
                         TmemPieces pieces{tacc + (hw + EPI_SETS * k) * EW::CH, EW::CH / PIECE, c.kb1 == c.kb0};
@@ -1950,12 +1963,14 @@ __device__ __forceinline__ void gemm_umma_body(const CUtensorMap& tmA, const CUt
                             ew.request(epp->bufs - 1u, row0, col(k - 1u + epp->bufs), c.z_out);
                         }
                         live_warp = ew.finish(c, row0, col(k), col(k) - colh, c.end, bias_row, pieces, read);
+                        stored();
                         if (!live_warp) break; // (a wait ran out: the abort flag ends the other roles)
                     }
                 }
             }
             ew.drain();
         }
+        if (warp == 2u && lane == 0) B200_TL(12);
     } else {
         // ------------------------------------------------------------------ epilogue
         const uint32_t q    = warp & 3u; // TMEM lane quarter this warp may read

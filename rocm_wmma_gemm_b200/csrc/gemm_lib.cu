@@ -1887,6 +1887,9 @@ extern "C" int b200_gemm_splitk_static(int types, void* C, const void* A, const 
 }
 
 #ifdef B200_GEMM_TIMELINE
+// (one translation unit, so that the stamps of all kernels go to the variables that are read here)
+#include "epilogue_kernels.cu"
+
 // Timeline builds only (see gemm_kernels.cuh): copies of the stamps, after a device synchronise
 // (b200_gemm_debug_reset clears them).
 // `out` holds TIMELINE_ROWS x TIMELINE_SLOTS values, `count` the launches stamped so far (row of

@@ -1,6 +1,7 @@
 """Where a GEMM launch spends its time: clock stamps from inside the kernels.
 
     python -m rocm_wmma_gemm_b200.timeline --type bf16_bf16 --shapes 1024,1024,1024 128,8192,8192
+    python -m rocm_wmma_gemm_b200.timeline --shapes 4096,4096,1024 --activation gelu_tanh
 
 loads the timeline build of the library (`build.py --timeline`: the same sources compiled with
 -DB200_GEMM_TIMELINE, whose kernels stamp clock64() at fixed points of the producer, MMA and
@@ -13,7 +14,8 @@ lists the points), replays each problem from a CUDA graph of back-to-back launch
   * how evenly the CTAs of the last launch ran: first load, end of the main loop and end of each
     CTA relative to the earliest first load.
 
-`B200_GEMM_CONFIG` and the other environment knobs of the library apply as usual.  The timeline
+`--activation` times the product with a bias and that activation (`b200_gemm_fused`) instead of the
+plain one.  `B200_GEMM_CONFIG` and the other environment knobs of the library apply as usual.  The timeline
 build is a profiling aid: its stamps cost a few global stores per launch, so its absolute times
 are a few per cent above the normal build's.
 """
@@ -25,7 +27,7 @@ import sys
 
 import numpy as np
 
-from . import build as lib_build
+from . import ACTIVATIONS, Epilogue, build as lib_build
 
 POINTS = ["entry", "set-up done", "dependency wait done", "first TMA load issued", "last TMA load issued",
           "first ring slot full", "last accumulator committed", "MMAs drained", "accumulator seen by epilogue",
@@ -43,13 +45,15 @@ def load() -> ctypes.CDLL:
         out, inp = name.split("_")
         fn = getattr(lib, f"b200_gemm_{out}_{inp}")
         fn.restype, fn.argtypes = ctypes.c_int, _ARGS
+    lib.b200_gemm_fused.restype = ctypes.c_int
+    lib.b200_gemm_fused.argtypes = [ctypes.c_int] + _ARGS + [ctypes.POINTER(Epilogue)]
     lib.b200_gemm_debug_timeline.restype = ctypes.c_int
     lib.b200_gemm_debug_cta_times.restype = ctypes.c_int
     lib.b200_gemm_debug_reset.restype = ctypes.c_int
     return lib
 
 
-def run(lib, type_name: str, M: int, N: int, K: int, layouts=(0, 1, 0), launches: int = 20) -> dict:
+def run(lib, type_name: str, M: int, N: int, K: int, layouts=(0, 1, 0), launches: int = 20, activation: str | None = None) -> dict:
     import torch
     la, lb, lc = layouts
     out_name, in_name = type_name.split("_")
@@ -60,9 +64,13 @@ def run(lib, type_name: str, M: int, N: int, K: int, layouts=(0, 1, 0), launches
     C = torch.empty(M * N, device="cuda", dtype=odt)
     fn_c = getattr(lib, f"b200_gemm_{out_name}_{in_name}")
 
+    bias = torch.rand(N, device="cuda").to(odt)
+    epi = Epilogue(ACTIVATIONS[activation], 0, bias.data_ptr(), None, None, None, 0) if activation else None
+
     def call():
         box = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-        st = fn_c(C.data_ptr(), A.data_ptr(), B.data_ptr(), M, N, K, 1, lc, la, lb, ctypes.byref(box))
+        args = (C.data_ptr(), A.data_ptr(), B.data_ptr(), M, N, K, 1, lc, la, lb, ctypes.byref(box))
+        st = lib.b200_gemm_fused(TYPES[type_name], *args, ctypes.byref(epi)) if epi else fn_c(*args)
         if st != 0:
             raise RuntimeError(f"b200_gemm_{out_name}_{in_name} returned {st}")
     for _ in range(3):
@@ -139,12 +147,14 @@ def main(argv=None) -> int:
     p.add_argument("--shapes", nargs="+", default=["1024,1024,1024"], help="M,N,K ...")
     p.add_argument("--layouts", default="r,c,r", help="A,B,C as r/c letters")
     p.add_argument("--launches", type=int, default=20, help="launches per CUDA graph")
+    p.add_argument("--activation", choices=list(ACTIVATIONS), help="the product with a bias and this activation")
     args = p.parse_args(argv)
     lay = tuple({"r": 0, "c": 1}[x] for x in args.layouts.split(","))
     lib = load()
     for s in args.shapes:
         M, N, K = (int(x) for x in s.split(","))
-        report(f"{M}x{N}x{K} {args.type} {args.layouts}", run(lib, args.type, M, N, K, lay, args.launches))
+        report(f"{M}x{N}x{K} {args.type} {args.layouts}" + (f" {args.activation}" if args.activation else ""),
+               run(lib, args.type, M, N, K, lay, args.launches, args.activation))
     return 0
 
 
