@@ -26,7 +26,8 @@ Inputs (>= 256 MB) are larger than the 126 MB L2, so no flush is needed between 
 is the same work through the host-buffer entry points (`b200_gemm_host`; `b200_gemm_slab_host`
 for N > 1: pinned host memory, host<->device copies inside the timed region).
 `--impl reference` times the reference's own CPU GEMM (test/test.hpp:59-129, compiled unmodified
-into oracle/_ref) on all host cores, on a bounded sample of rows of the same workload.
+into oracle/_ref) on all host cores, on a bounded sample of rows of the same workload; where
+that is not built it says so (`unavailable`).
 """
 from __future__ import annotations
 
@@ -183,6 +184,10 @@ def cpu_baseline(workload, target_s=12.0):
 
 def run_reference(args, rank, world):
     if rank != 0:
+        return
+    import oracle
+    if oracle.ref_lib() is None:  # (the oracle's restatement is not the reference)
+        emit_line({"impl": "reference", "unavailable": "no reference checkout to compile its CPU GEMM from (oracle/_ref is not built)"})
         return
     workload = workload_for(args.gpus)
     types, M, N, K, (la, lb, lc), sigma = workload["cpu"]
