@@ -267,7 +267,8 @@ int b200_gemm_slab_host(b200_gemm_comm* comm, int types, void* C_slab, const voi
  * Everything after the product is computed in f32 from the f32 accumulators and rounded once,
  * when C and Z are stored: C is rounded from act of the unrounded Z, the gradient takes the
  * stored (rounded) Z.  Activations and slopes hold over the whole range of the types: at the
- * infinities they are their limits (act(inf) = inf, act(-inf) = 0, slopes 1 and 0), a NaN stays a NaN.
+ * infinities they are their limits (act(inf) = inf, act(-inf) = 0, slopes 1 and 0; ACT_NONE passes Z
+ * on), a NaN stays a NaN.
  * The bias gradient is always f32, summed in a fixed order (equal inputs give
  * equal bits).  bias, residual, preact and C share C's element type; residual and preact are
  * matrices of C's shape, layout and batch stride.
